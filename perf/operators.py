@@ -10,8 +10,8 @@ Three operators that a step of such work is made of:
 A case's keys.  ``attention``: ``groups`` of up to ``beams`` sequences (``ragged``: from 1 to ``beams``), ``shared`` keys (``ragged``:
 from half of it up), up to ``own`` keys of a sequence's own; ``heads``, ``kv_heads``, ``head_dim``, ``dtype``, ``page``, ``sinks``.
 ``select``: ``requests``, ``beams``, ``vocab``, ``keep``, ``masked`` (one token in so many is forbidden; 0: none), ``first`` (a
-request's first step: one beam alone has begun).  ``reorder``: ``requests``, ``beams``, ``rows`` per beam, ``layers`` tensors of
-``width`` elements a row, ``dtype``.
+request's first step: one beam alone has begun).  ``reorder``: ``requests``, ``beams``, ``rows`` per beam, ``layers`` of
+``width`` elements a row, ``dtype``; the layers' rows lie in one tensor, as a page group's do.
 """
 from __future__ import annotations
 
@@ -213,7 +213,7 @@ def _own(s):
                                            s["group_starts"], s["shared_lens"], s["largest"], s["longest"], s["scale"], workspace, sinks=s["sinks"])
     if case["op"] == "select":
         return ops.beam_select(s["logits"], s["scores"], case["keep"])
-    ops.reorder_states(list(s["states"].unbind(0)), s["slots"], s["parents"])
+    ops.reorder_states([s["states"]], s["slots"], s["parents"], axis=1)
     return s["states"]
 
 
