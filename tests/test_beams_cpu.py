@@ -1,0 +1,163 @@
+"""What the operators for several continuations of one prompt refuse, before anything is launched."""
+import math
+
+import pytest
+import torch
+
+from velox_amd.kernels.hip_ops import HipOps, KernelError
+
+
+class _Nothing:
+    def __getattr__(self, name):
+        raise AssertionError(f"{name} was reached")
+
+
+@pytest.fixture()
+def ops():
+    """The checks alone: no library, so that anything that passes them says so."""
+    made = object.__new__(HipOps)
+    made.device = torch.device("cpu")
+    made.num_cus = 256
+    made._raw_stream = None
+    made._shared_prefix = {dim: _Nothing() for dim in range(16, 272, 16)}
+    made._beams = _Nothing()
+    return made
+
+
+class _Workspace:
+    def get(self, name, numel):
+        return torch.empty(numel)
+
+
+def attention(**changed):
+    a = dict(qkv=torch.zeros((3, 8 * 64)), num_heads=4, num_kv_heads=2, head_dim=64, k_cache=torch.zeros((9, 2, 16, 64)), v_cache=torch.zeros((9, 2, 64, 16)), block_size=16,
+             block_tables=torch.zeros((3, 4), dtype=torch.int32), kv_lens=torch.ones(3, dtype=torch.int32), group_starts=torch.tensor([0, 3], dtype=torch.int32),
+             shared_lens=torch.tensor([1], dtype=torch.int32), largest_group=3, max_kv_len=64, scale=0.125, workspace=_Workspace())
+    a.update(changed)
+    return a
+
+
+@pytest.mark.parametrize("changed,says", [
+    (dict(qkv=torch.zeros((3, 8 * 64), dtype=torch.float16)), "float32 or bfloat16"),
+    (dict(qkv=torch.zeros((3, 8 * 64 + 1))), "rows of"),
+    (dict(qkv=torch.zeros((4, 8 * 64))), "qkv"),
+    (dict(qkv=torch.zeros((3, 16 * 64))[:, ::2]), "contiguous"),
+    (dict(num_heads=5), "multiple"),
+    (dict(num_kv_heads=0), "multiple"),
+    (dict(head_dim=60), "head_dim"),
+    (dict(head_dim=512), "head_dim"),
+    (dict(k_cache=torch.zeros((9, 2, 16, 64), dtype=torch.bfloat16)), "k_cache"),
+    (dict(k_cache=torch.zeros((0, 2, 16, 64))), "without pages"),
+    (dict(v_cache=torch.zeros((9, 2, 16, 64))), "v_cache"),
+    (dict(block_size=4), "block_size"),
+    (dict(block_size=24), "block_size"),
+    (dict(block_tables=torch.zeros((2, 4), dtype=torch.int32)), "block_tables"),
+    (dict(block_tables=torch.zeros((3, 4), dtype=torch.int64)), "block_tables"),
+    (dict(max_kv_len=65), "cannot cover"),
+    (dict(max_kv_len=-1), "cannot cover"),
+    (dict(kv_lens=torch.ones(3, dtype=torch.int64)), "kv_lens"),
+    (dict(kv_lens=torch.ones((3, 1), dtype=torch.int32)), "kv_lens"),
+    (dict(group_starts=torch.tensor([0, 1, 3], dtype=torch.int32)), "starts"),
+    (dict(shared_lens=torch.tensor([[1]], dtype=torch.int32)), "starts"),
+    (dict(group_starts=torch.zeros(1026, dtype=torch.int32), shared_lens=torch.zeros(1025, dtype=torch.int32)), "at most 1024"),
+    (dict(largest_group=0), "largest group"),
+    (dict(largest_group=4), "largest group"),
+    (dict(scale=0.0), "scale"),
+    (dict(scale=math.nan), "scale"),
+    (dict(sinks=torch.zeros(5)), "sinks"),
+    (dict(sinks=torch.zeros(4, dtype=torch.bfloat16)), "sinks"),
+    (dict(workspace=None), "workspace"),
+])
+def test_attention_refuses(ops, changed, says):
+    with pytest.raises(KernelError, match=says):
+        ops.shared_prefix_attention(**attention(**changed))
+
+
+def test_attention_of_no_sequences(ops):
+    out = ops.shared_prefix_attention(**attention(qkv=torch.zeros((0, 8 * 64)), block_tables=torch.zeros((0, 4), dtype=torch.int32), kv_lens=torch.zeros(0, dtype=torch.int32),
+                                                  group_starts=torch.zeros(1, dtype=torch.int32), shared_lens=torch.zeros(0, dtype=torch.int32), largest_group=1))
+    assert out.shape == (0, 256)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(28, 4, 128), (12, 2, 128), (32, 1, 64), (8, 8, 256), (3, 1, 16)])
+def test_attention_items_are_enough(ops, heads, kv_heads, dim):
+    """The bound on the items that the launch has room for, against the kernels' own count, over lengths and groups at random."""
+    import random
+
+    rng = random.Random(heads)
+    group = heads // kv_heads
+    for _ in range(300):
+        sizes = [rng.choice([0, 1, 2, 3, 17, 70]) for _ in range(rng.randint(0, 9))]
+        num_seqs = max(1, sum(sizes) + rng.randint(0, 5))
+        row_tiles, target, items = ops._shared_prefix_shape(num_seqs, len(sizes), heads, kv_heads, dim, rng.choice([2, 4]), max(sizes + [1]))
+        steps = lambda low, high: -(-(high - low // 32 * 32) // 128) if high > low else 0  # noqa: E731
+        work = []  # (row blocks, steps)
+        b = 0
+        for size in sizes:
+            shared = rng.choice([0, 1, 5, 128, 1000, 33333]) if size > 1 else 0
+            if shared:
+                work.append((-(-size * group // (16 * row_tiles)), steps(0, shared)))
+            work += [(-(-group // 16), steps(shared, shared + rng.choice([0, 1, 200, 5000]))) for _ in range(size)]
+            b += size
+        work += [(-(-group // 16), steps(0, rng.choice([0, 1, 200, 5000]))) for _ in range(num_seqs - b)]
+        per = max(1, -(-sum(x * y for x, y in work) // target))
+        assert sum(x * -(-y // per) for x, y in work) <= items
+
+
+@pytest.mark.parametrize("logits,scores,keep,says", [
+    (torch.zeros((4, 9), dtype=torch.bfloat16), torch.zeros((2, 2)), 4, "logits"),
+    (torch.zeros((4, 9)).double(), torch.zeros((2, 2)), 4, "logits"),
+    (torch.zeros((4, 18))[:, ::2], torch.zeros((2, 2)), 4, "contiguous"),
+    (torch.zeros((4, 9)), torch.zeros((2, 2)).double(), 4, "scores"),
+    (torch.zeros((4, 9)), torch.zeros((2, 3)), 4, "do not go"),
+    (torch.zeros((4, 9)), torch.zeros(4), 4, "do not go"),
+    (torch.zeros((4, 9)), torch.zeros((2, 2)), 0, "keep"),
+    (torch.zeros((4, 9)), torch.zeros((2, 2)), 19, "keep"),
+    (torch.zeros((4, 99)), torch.zeros((2, 2)), 65, "keep"),
+    (torch.zeros((257, 9)), torch.zeros((1, 257)), 4, "beams"),
+    (torch.zeros((4, 0)), torch.zeros((2, 2)), 1, "tokens"),
+    (torch.zeros((0, 9)), torch.zeros((2, 0)), 1, "beams"),
+    (torch.zeros((65536, 1)), torch.zeros((65536, 1)), 1, "grid"),
+])
+def test_selection_refuses(ops, logits, scores, keep, says):
+    with pytest.raises(KernelError, match=says):
+        ops.beam_select(logits, scores, keep)
+
+
+def test_selection_of_no_requests(ops):
+    values, parents, tokens = ops.beam_select(torch.zeros((0, 9)), torch.zeros((0, 2)), 4)
+    assert values.shape == parents.shape == tokens.shape == (0, 4) and parents.dtype == tokens.dtype == torch.int32
+
+
+def ints(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("tensors,slots,parents,axis,says", [
+    ([torch.zeros((9, 4))], ints([0, 1]).long(), ints([0, 1]), 0, "slots"),
+    ([torch.zeros((9, 4))], ints([0, 1]), ints([0, 1]).long(), 0, "parents"),
+    ([torch.zeros((9, 4))], ints([0, 1]), ints([0, 1, 2]), 0, "do not go"),
+    ([torch.zeros((9, 4))], ints(0, 1), ints(0, 1), 0, "do not go"),
+    ([torch.zeros((9, 4))], torch.zeros((1, 65), dtype=torch.int32), torch.zeros((1, 65), dtype=torch.int32), 0, "beams"),
+    ([torch.zeros((9, 4))], torch.zeros((1, 2, 65536), dtype=torch.int32), ints([0, 1]), 0, "rows"),
+    ([torch.zeros((9, 4))], ints([0, 1]), ints([0, 1]), 2, "dimension"),
+    ([torch.zeros((9, 4))], ints([0, 1]), ints([0, 1]), -1, "dimension"),
+    ([torch.zeros((9, 8))[:, ::2]], ints([0, 1]), ints([0, 1]), 0, "contiguous"),
+    ([torch.zeros((65536, 9, 1))], ints([0, 1]), ints([0, 1]), 1, "grid"),
+])
+def test_reorder_refuses(ops, tensors, slots, parents, axis, says):
+    with pytest.raises(KernelError, match=says):
+        ops.reorder_states(tensors, slots, parents, axis=axis)
+
+
+def test_reorder_refuses_shared_memory(ops):
+    t = torch.zeros((9, 4))
+    for pair in ([t, t], [t, t[3:]], [t[:5], t[4:]]):
+        with pytest.raises(KernelError, match="share memory"):
+            ops.reorder_states(pair, ints([0, 1]), ints([0, 1]))
+
+
+def test_reorder_of_nothing(ops):
+    ops.reorder_states([], ints([0, 1]), ints([1, 0]))
+    ops.reorder_states([torch.zeros((9, 0))], ints([0, 1]), ints([1, 0]))
+    ops.reorder_states([torch.zeros((9, 4))], torch.zeros((0, 2), dtype=torch.int32), torch.zeros((0, 2), dtype=torch.int32))

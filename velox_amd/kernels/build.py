@@ -1,7 +1,8 @@
 """Compiles the HIP sources under ``velox_amd/csrc`` for gfx950 into shared libraries and finds them again.
 
-Two kinds of library: ``core`` (everything whose sizes are run-time arguments) and ``attn_d<N>``
-(the attention kernels for one head size, a compile-time constant).  A library's file name
+Kinds of library: ``core`` (what every model runs and whose sizes are run-time arguments), ``attn_d<N>`` (the attention
+kernels for one head size, a compile-time constant), ``prefix_d<N>`` (attention over shared prefixes, likewise) and
+``beams`` (several continuations of a request).  A library's file name
 carries a hash of the sources and flags it was built from, so a stale build is never loaded.
 Libraries are built in-tree (``velox_amd/_build``) when that folder can be written, otherwise
 under ``$VELOX_AMD_BUILD_DIR``, the user's cache folder or the temporary folder.  A build
@@ -25,6 +26,8 @@ ARCH = "gfx950"
 FLAGS = ["-O3", f"--offload-arch={ARCH}", "-shared", "-fPIC", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 CORE_SOURCES = ["elementwise.hip", "gemm.hip", "split_f32.hip", "skinny_gemm.hip", "latent.hip", "routed.hip", "normed.hip", "recurrent.hip", "removal.hip", "linear_chunk.hip", "state_space.hip", "gated.hip", "sampling.hip", "probe.hip"]
 ATTENTION_SOURCES = ["attention.hip"]
+SHARED_PREFIX_SOURCES = ["shared_prefix.hip"]
+BEAM_SOURCES = ["beams.hip"]
 HEADERS = ["common.h", "no_alloc.h", "grouped_mfma.h", "tiles_mfma.h"]
 # head sizes built ahead of time by build_all(); any other multiple of 16 up to 256 is built at first use
 DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 192, 256)
@@ -185,6 +188,21 @@ def ensure_attention(head_dim: int, force: bool = False, biased: bool = False, k
     return ensure_library(stem, sources, defines, force)
 
 
+def _shared_prefix_job(head_dim: int):
+    return f"prefix_d{head_dim}", SHARED_PREFIX_SOURCES, {"VELOX_HEAD_DIM": head_dim}
+
+
+def ensure_shared_prefix(head_dim: int, force: bool = False) -> str:
+    if head_dim % 16 != 0 or not 16 <= head_dim <= 256:
+        raise BuildError(f"head_dim={head_dim}: attention over shared prefixes takes multiples of 16 from 16 to 256")
+    stem, sources, defines = _shared_prefix_job(head_dim)
+    return ensure_library(stem, sources, defines, force)
+
+
+def ensure_beams(force: bool = False) -> str:
+    return ensure_library("beams", BEAM_SOURCES, {}, force)
+
+
 def build_all(head_dims: Sequence[int] = DEFAULT_HEAD_DIMS, force: bool = True, biased_head_dims: Sequence[int] = DEFAULT_BIASED_HEAD_DIMS,
               optioned_heads: Sequence[tuple] = DEFAULT_OPTIONED_HEADS) -> List[str]:
     """Compiles every library (in parallel, one hipcc per library)."""
@@ -192,5 +210,6 @@ def build_all(head_dims: Sequence[int] = DEFAULT_HEAD_DIMS, force: bool = True, 
 
     jobs = [("core", CORE_SOURCES, {})] + [_attention_job(d, "") for d in head_dims] + [_attention_job(d, "b") for d in biased_head_dims]
     jobs += [_attention_job(d, options) for d, options in optioned_heads]
+    jobs += [("beams", BEAM_SOURCES, {})] + [_shared_prefix_job(d) for d in head_dims]
     with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as pool:
         return list(pool.map(lambda job: ensure_library(job[0], job[1], job[2], force), jobs))

@@ -106,6 +106,8 @@ class HipOps:
             raise KernelError(f"the kernels are built for {build.ARCH}; this GPU is {arch}")
         self._core = ctypes.CDLL(build.ensure_core())
         self._attention: Dict[Tuple[int, str], ctypes.CDLL] = {}
+        self._shared_prefix: Dict[int, ctypes.CDLL] = {}
+        self._beams: Optional[ctypes.CDLL] = None
         self._declare_core()
         self.num_cus = torch.cuda.get_device_properties(self.device).multi_processor_count
         self.use_library_gemm = True
@@ -269,6 +271,34 @@ class HipOps:
             self._attention[key] = lib
         return lib
 
+    def shared_prefix_library(self, head_dim: int) -> ctypes.CDLL:
+        """The kernels of ``shared_prefix_attention`` for one head size."""
+        lib = self._shared_prefix.get(head_dim)
+        if lib is None:
+            lib = ctypes.CDLL(build.ensure_shared_prefix(head_dim))
+            lib.velox_shared_prefix_attention.argtypes = [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P, _P, _I, _P]
+            lib.velox_shared_prefix_most_row_tiles.argtypes = [_I]
+            for fn in (lib.velox_shared_prefix_attention, lib.velox_shared_prefix_most_row_tiles, lib.velox_shared_prefix_head_dim):
+                fn.restype = _I
+            if lib.velox_shared_prefix_head_dim() != head_dim:
+                raise KernelError(f"shared-prefix library for head_dim={head_dim} reports {lib.velox_shared_prefix_head_dim()}")
+            self._shared_prefix[head_dim] = lib
+        return lib
+
+    def beam_library(self) -> ctypes.CDLL:
+        """The kernels of ``beam_select`` and ``reorder_states``."""
+        if self._beams is None:
+            lib = ctypes.CDLL(build.ensure_beams())
+            lib.velox_beam_pieces.argtypes = [_I, _I]
+            lib.velox_beam_scratch_bytes.argtypes = [_I, _I, _I]
+            lib.velox_beam_scratch_bytes.restype = ctypes.c_longlong
+            lib.velox_beam_select.argtypes = [_P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _P, _P, _P]
+            lib.velox_reorder_states.argtypes = [_P, _I, _P, _P, _I, _I, _I, _P]
+            for fn in (lib.velox_beam_pieces, lib.velox_beam_select, lib.velox_reorder_states):
+                fn.restype = _I
+            self._beams = lib
+        return self._beams
+
     def prepare(self, model, dtype) -> None:
         """Lets every part get what it needs of the kernels before the first step (``Part.prepare_kernels``): the weights
         that decode-sized products read are registered, and libraries that are built per size (attention, per head
@@ -380,6 +410,10 @@ class HipOps:
         if self._raw_stream is not None:
             return _P(self._raw_stream(self.device.index))
         return _P(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _current(self):
+        """The kernels' device as the current one (a launch goes to the current device's queues)."""
+        return contextlib.nullcontext() if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
 
     def _check(self, name: str, t: torch.Tensor, dtype=None, shape=None, align: int = 4) -> None:
         if not isinstance(t, torch.Tensor) or t.device != self.device:
@@ -2261,6 +2295,178 @@ class HipOps:
         else:
             launch(0, num_seqs, 0, tokens, max_q_len, bool(all_decode), splits)
         return out
+
+    # -- several continuations of one prompt ------------------------------------------------------
+    MAX_PREFIX_GROUPS = 1024  # of one call of ``shared_prefix_attention``
+    MAX_BEAMS, MAX_KEPT, MAX_BEAM_VOCAB = 256, 64, 1 << 24  # of ``beam_select``
+    MAX_MOVED = 64  # beams of a request that ``reorder_states`` moves
+
+    def _shared_prefix_shape(self, num_seqs: int, num_groups: int, num_heads: int, num_kv_heads: int, head_dim: int, element_size: int, largest_group: int) -> Tuple[int, int, int]:
+        """Row tiles of a workgroup, over how many workgroups per KV head the keys are cut, and the most items that makes."""
+        group = num_heads // num_kv_heads
+        most = 4 if element_size * head_dim <= 256 else 2 if element_size * head_dim <= 512 else 1
+        row_tiles = 1
+        while row_tiles < most and 16 * row_tiles < largest_group * group:
+            row_tiles *= 2
+        target = max(1, self.num_cus // num_kv_heads)
+        return row_tiles, target, target + num_seqs * group // (16 * row_tiles) + num_groups + num_seqs * (-(-group // 16))
+
+    def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> Tuple[int, int]:
+        """The most float32 elements ``shared_prefix_attention`` asks its workspace for (``shared_prefix_out``, ``shared_prefix_lse``) in any
+        step of at most so many sequences and groups, whatever the lengths and the element type."""
+        rows = 0
+        for element_size in (2, 4):
+            for largest in (1, 1 << 20):
+                row_tiles, _, items = self._shared_prefix_shape(max_num_seqs, max_num_groups, num_heads, num_kv_heads, head_dim, element_size, largest)
+                rows = max(rows, items * num_kv_heads * 16 * row_tiles)
+        return rows * head_dim, rows
+
+    def shared_prefix_attention(self, qkv, num_heads, num_kv_heads, head_dim, k_cache, v_cache, block_size, block_tables, kv_lens, group_starts, shared_lens,
+                                largest_group, max_kv_len, scale, workspace, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of a decode step whose sequences share their first keys in groups: the shared keys are read once per group, and not once per
+        sequence as by ``paged_attention``, whose arguments these are otherwise.  One token per sequence (row ``b`` of ``qkv``).
+
+        Group ``g`` is sequences ``group_starts[g] .. group_starts[g + 1] - 1`` (int32 ``[groups + 1]``, rising); the first ``shared_lens[g]``
+        keys (int32 ``[groups]``; any number, pages need not be full) of each of them are the same ones, and are read through
+        the block table of the group's FIRST sequence.  What a sequence has behind them is read through its own table, whose entries for
+        pages that hold shared keys only are not looked at.  Sequences outside every group, alone in one, or with fewer keys than their group
+        shares share nothing; a group shares no more keys than its first sequence has.  A sequence without keys gets zeros.
+        ``largest_group``: sequences of the largest group (which kernel is launched goes by it, the result does not), ``max_kv_len``: the most keys
+        of any sequence (a greater length counts as that many).  Lengths and groups are read on the device only: a captured call replays with other ones, as long as the number of
+        sequences and groups stays.  ``sinks``: as for ``paged_attention``.  Pages hold at least 8 tokens."""
+        num_seqs = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+        width = qkv.shape[1] if qkv.dim() == 2 else -1
+        if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads != 0:
+            raise KernelError("num_heads must be a multiple of num_kv_heads")
+        if head_dim % 16 != 0 or not 16 <= head_dim <= self.MAX_TILED_HEAD_DIM:
+            raise KernelError(f"shared_prefix_attention: head_dim={head_dim} is no multiple of 16 up to {self.MAX_TILED_HEAD_DIM}")
+        if width not in (num_heads * head_dim, (num_heads + 2 * num_kv_heads) * head_dim):
+            raise KernelError(f"shared_prefix_attention: rows of {width} elements hold neither the queries nor queries, keys and values")
+        dtype = _code(qkv.dtype)
+        self._check("kv_lens", kv_lens, torch.int32, (num_seqs,))
+        self._check("qkv", qkv, None, (num_seqs, width), align=16)
+        self._check("group_starts", group_starts, torch.int32)
+        self._check("shared_lens", shared_lens, torch.int32)
+        num_groups = shared_lens.numel()
+        if shared_lens.dim() != 1 or tuple(group_starts.shape) != (num_groups + 1,) or num_groups > self.MAX_PREFIX_GROUPS:
+            raise KernelError(f"shared_prefix_attention: {tuple(group_starts.shape)} starts do not go with {tuple(shared_lens.shape)} groups, at most {self.MAX_PREFIX_GROUPS}")
+        self._check("block_tables", block_tables, torch.int32)
+        if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs:
+            raise KernelError(f"block_tables must be [{num_seqs}, W], got {tuple(block_tables.shape)}")
+        if block_size < 8 or block_size & (block_size - 1):
+            raise KernelError(f"shared_prefix_attention: block_size must be a power of two from 8 on, got {block_size}")
+        if max_kv_len < 0 or block_tables.shape[1] * block_size < max_kv_len:
+            raise KernelError(f"block tables of width {block_tables.shape[1]} cannot cover {max_kv_len} keys")
+        pages = k_cache.shape[0]
+        if pages < 1:
+            raise KernelError("shared_prefix_attention: a cache without pages")
+        self._check("k_cache", k_cache, qkv.dtype, (pages, num_kv_heads, block_size, head_dim), align=16)
+        self._check("v_cache", v_cache, qkv.dtype, (pages, num_kv_heads, head_dim, block_size), align=16)
+        if not 0 < scale < float("inf"):
+            raise KernelError(f"shared_prefix_attention: the scale must be positive, got {scale}")
+        if sinks is not None:
+            self._check("sinks", sinks, torch.float32, (num_heads,))
+        if not 1 <= largest_group <= max(num_seqs, 1):
+            raise KernelError(f"shared_prefix_attention: a largest group of {largest_group} among {num_seqs} sequences")
+        if workspace is None:
+            raise KernelError("shared_prefix_attention needs a workspace")
+        out = torch.empty((num_seqs, num_heads * head_dim), dtype=qkv.dtype, device=self.device)
+        if num_seqs == 0:
+            return out
+        row_tiles, target, items = self._shared_prefix_shape(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, qkv.element_size(), int(largest_group))
+        if items > 65535 or num_seqs > 65535:
+            raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
+        rows = items * num_kv_heads * 16 * row_tiles
+        part_o = workspace.get("shared_prefix_out", rows * head_dim)
+        part_lse = workspace.get("shared_prefix_lse", rows)
+        lib = self.shared_prefix_library(head_dim)
+        with self._current():
+            status = lib.velox_shared_prefix_attention(
+                _ptr(qkv), width, _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(kv_lens), _ptr(group_starts), _ptr(shared_lens), num_seqs,
+                num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages, int(max_kv_len), float(scale), row_tiles, target, items, _ptr(sinks), _ptr(out), _ptr(part_o), _ptr(part_lse),
+                dtype, self._stream())
+        self._launched(status, "shared_prefix_attention")
+        return out
+
+    def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, keep: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The ``keep`` best continuations of every request over its beams and the vocabulary.  ``logits`` float32 ``[requests * beams, vocab]``,
+        ``scores`` float32 ``[requests, beams]``, the beams' sums of log-probabilities (-inf: a beam that is not there).  A continuation of beam ``w``
+        by token ``v`` is worth ``scores[w] + log_softmax(logits[w])[v]``, in 64 bits.  Returns, best first, their values (float32), their beams
+        and their tokens (int32), each ``[requests, keep]``.  Equal ones come by the lowest beam, then by the greater logit, then by the lowest token;
+        a logit that is -inf or no number makes a value of -inf, and those come last."""
+        self._check("logits", logits, torch.float32)
+        self._check("scores", scores, torch.float32)
+        if logits.dim() != 2 or scores.dim() != 2 or scores.numel() != logits.shape[0]:
+            raise KernelError(f"beam_select: {tuple(scores.shape)} scores do not go with logits of shape {tuple(logits.shape)}")
+        (requests, beams), vocab, keep = scores.shape, logits.shape[1], int(keep)
+        if not 1 <= beams <= self.MAX_BEAMS or not 1 <= vocab <= self.MAX_BEAM_VOCAB:
+            raise KernelError(f"beam_select: {beams} beams over {vocab} tokens; 1 to {self.MAX_BEAMS} and 1 to {self.MAX_BEAM_VOCAB} are taken")
+        if not 1 <= keep <= min(self.MAX_KEPT, beams * vocab):
+            raise KernelError(f"beam_select: keep={keep} is not between 1 and {min(self.MAX_KEPT, beams * vocab)}")
+        rows = requests * beams
+        if rows > 65535:
+            raise KernelError(f"beam_select: {rows} rows exceed the launch grid")
+        values = torch.empty((requests, keep), dtype=torch.float32, device=self.device)
+        parents = torch.empty((requests, keep), dtype=torch.int32, device=self.device)
+        tokens = torch.empty((requests, keep), dtype=torch.int32, device=self.device)
+        if requests == 0:
+            return values, parents, tokens
+        lib = self.beam_library()
+        per_thread = 32 if rows * lib.velox_beam_pieces(vocab, 32) >= 2 * self.num_cus else 8
+        size = int(lib.velox_beam_scratch_bytes(rows, lib.velox_beam_pieces(vocab, per_thread), keep))
+        scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
+        with self._current():
+            status = lib.velox_beam_select(_ptr(logits), _ptr(scores), requests, beams, vocab, keep, per_thread, _ptr(scratch), size, _ptr(values), _ptr(parents), _ptr(tokens),
+                                           self._stream())
+        self._launched(status, "beam_select")
+        return values, parents, tokens
+
+    def reorder_states(self, tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents: torch.Tensor, axis: int = 0) -> None:
+        """Every beam takes over what its parent held, in place: row ``slots[b, j, p]`` along dimension ``axis`` of every tensor becomes what row
+        ``slots[b, parents[b, j], p]`` was before the call.  ``slots`` int32 ``[requests, beams]`` or ``[requests, beams, rows]`` (state slots, or the pages behind
+        a shared prefix), ``parents`` int32 ``[requests, beams]``, at most ``MAX_MOVED`` beams.  A row or a parent outside its range (-1: none) moves nothing
+        and is not moved to.  Every row belongs to one beam of one request, and the tensors share no memory."""
+        self._check("slots", slots, torch.int32)
+        self._check("parents", parents, torch.int32)
+        if parents.dim() != 2 or slots.dim() not in (2, 3) or slots.shape[:2] != parents.shape:
+            raise KernelError(f"reorder_states: slots of shape {tuple(slots.shape)} do not go with parents of shape {tuple(parents.shape)}")
+        requests, beams = parents.shape
+        places = slots.shape[2] if slots.dim() == 3 else 1
+        if not 1 <= beams <= self.MAX_MOVED or requests * places > 65535:
+            raise KernelError(f"reorder_states: {requests} requests of {beams} beams with {places} rows; 1 to {self.MAX_MOVED} beams and 65,535 rows of a beam are taken")
+        described, spans = [], []
+        for at, t in enumerate(tensors):
+            self._check(f"tensors[{at}]", t, align=1)
+            if not 0 <= axis < t.dim():
+                raise KernelError(f"reorder_states: tensors[{at}] of shape {tuple(t.shape)} has no dimension {axis}")
+            if t.numel() == 0:
+                continue
+            outer, rows = 1, t.shape[axis]
+            for n in t.shape[:axis]:
+                outer *= n
+            run = t.numel() // outer * t.element_size()
+            if outer > 65535 or rows > 0x7FFFFFFF:
+                raise KernelError(f"reorder_states: tensors[{at}] of shape {tuple(t.shape)} exceeds the launch grid")
+            start = t.data_ptr()
+            described.append((start, outer, run, rows, run // rows))
+            spans.append((start, start + outer * run))
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise KernelError("reorder_states: two tensors share memory")
+        if requests * places == 0 or not described:
+            return
+        lib = self.beam_library()
+        at = 0
+        with self._current():
+            while at < len(described):  # up to 32 tensors and 65,535 runs of rows a launch
+                end, runs = at, 0
+                while end < len(described) and end - at < 32 and runs + described[end][1] <= 65535:
+                    runs += described[end][1]
+                    end += 1
+                numbers = [n for d in described[at:end] for n in d]
+                status = lib.velox_reorder_states((ctypes.c_longlong * len(numbers))(*numbers), end - at, _ptr(slots), _ptr(parents), requests, beams, places, self._stream())
+                self._launched(status, "reorder_states")
+                at = end
 
     # -- sampling -------------------------------------------------------------------------------
     def argmax(self, logits: torch.Tensor) -> torch.Tensor:
