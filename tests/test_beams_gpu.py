@@ -324,6 +324,25 @@ def test_select_beams_that_are_not_there(ops, vocab):
     check_selection(ops, logits, scores, 12)
 
 
+@pytest.mark.parametrize("absent", [range(0, 100), range(100, 200), range(0, 200, 2)])
+def test_select_many_lists_of_which_many_are_empty(ops, absent):
+    logits, scores = random_case(2, 200, 1021)
+    scores[1, list(absent)] = -math.inf
+    check_selection(ops, logits, scores, 64)
+
+
+@pytest.mark.parametrize("keep", [4, 16, 17, 64])
+def test_select_most_of_a_piece_alike(ops, keep):
+    """More equal ones than are ranked: places decide."""
+    g = torch.Generator().manual_seed(4)
+    logits = torch.zeros((6, 20000))
+    logits[1] = (torch.arange(20000) > 12000).float()
+    logits[2, 5000:] = -math.inf
+    logits[3, ::2] = 1.0
+    logits[4] = torch.randn(20000, generator=g).round()
+    check_selection(ops, logits, torch.zeros((3, 2)), keep)
+
+
 @pytest.mark.parametrize("vocab,keep", [(40, 10), (2500, 64), (9001, 20)])
 def test_select_ties(ops, vocab, keep):
     """Equal logits in a row, equal rows, zeros of both signs."""

@@ -7,9 +7,11 @@
 // bits would change the order of near ones: sums and values are held in 64 bits.  One kernel reads the logits once, a piece of a row per
 // workgroup, and leaves each piece's maximum, sum of exponentials and best `keep` in order; a second, one workgroup per request, joins them.
 //
-// A piece's best `keep`.  Every value gets a key that no other of the piece has: its bits in an order that compares like numbers, then
-// its place counted from the end.  The `keep`-th largest among the maxima of disjoint parts of the piece is not above the `keep`-th
-// largest key of all, and at most `keep` parts hold keys as large: only those keys, a few more than `keep` as a rule, are ranked.
+// A piece's best `keep`.  Each of a workgroup's four waves keeps a list of what may be wanted of the values it has seen.  It has two bounds: one that
+// `keep` values of its own reach, the least of the maxima of as many groups of lanes, which a value must exceed to join the list (an
+// equal one comes behind those that set the bound), and the least of the four waves' bounds for a quarter of `keep`, which it must reach.  Joining is soon the
+// exception; a list that is full is cut to its best `keep`.  The waves read what bounds the others have published and wait for one
+// another behind the first round alone.
 //
 // reorder_states: row slots[b, j, p] of every tensor becomes what row slots[b, parents[b, j], p] was.  A thread owns a column of the rows of one
 // request: it has read all that move before it writes any, and nobody else reads or writes that column, so the rows change places
@@ -20,23 +22,27 @@
 constexpr int THREADS = 256;
 constexpr int MOST_KEPT = 64;
 
-// exp(x) for x <= 0 in 64 bits, to 1e-11 of it: x = k ln 2 + r with |r| <= ln 2 / 2, and the series of e^r to its ninth power
-// (the next term is at most 0.347^10 / 10! = 7e-12).
-__device__ __forceinline__ double exp_below_zero(double x) {
-  const double k = rint(x * 1.4426950408889634074);
-  const double r = fma(k, -0.69314718055994530942, x);
-  double e = 1.0 / 362880.0;
-  e = fma(e, r, 1.0 / 40320.0);
-  e = fma(e, r, 1.0 / 5040.0);
-  e = fma(e, r, 1.0 / 720.0);
-  e = fma(e, r, 1.0 / 120.0);
-  e = fma(e, r, 1.0 / 24.0);
-  e = fma(e, r, 1.0 / 6.0);
-  e = fma(e, r, 0.5);
-  e = fma(e, r, 1.0);
-  e = fma(e, r, 1.0);
-  return x < -700.0 ? 0.0 : ldexp(e, (int)k);
+// 2^t for -1000 <= t <= 1000 in 64 bits, to 6e-11 of it: t = k + f with |f| <= 1/2, and the polynomial of degree 7 that takes 2^f's values at the
+// Chebyshev points of that range.  (Adding 1.5 2^52 leaves k in the sum's low bits; it goes into the exponent.)
+__device__ __forceinline__ double exp2_near_zero(double t) {
+  const double shifted = t + 6755399441055744.0, f = t - (shifted - 6755399441055744.0);
+  double e = 1.5303699001378845e-05;
+  e = fma(e, f, 0.00015469729140704658);
+  e = fma(e, f, 0.0013333478480888061);
+  e = fma(e, f, 0.0096180256135980358);
+  e = fma(e, f, 0.055504109063177154);
+  e = fma(e, f, 0.24022651213495422);
+  e = fma(e, f, 0.69314718055683411);
+  e = fma(e, f, 0.99999999995956224);
+  typedef uint32_t halves_t __attribute__((ext_vector_type(2)));
+  halves_t bits = __builtin_bit_cast(halves_t, e);
+  bits[1] += __builtin_bit_cast(halves_t, shifted)[0] << 20;
+  return __builtin_bit_cast(double, bits);
 }
+// the greater of the two, `a` if b is no number (one instruction; fmaxf takes another to quiet its operands)
+__device__ __forceinline__ float greater(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+constexpr double LOG2_E = 1.4426950408889634074;
+constexpr float FAR_BELOW = 690.f;  // from here on a term is nothing beside 1
 
 __device__ __forceinline__ uint32_t ordered_bits(float v) {  // compares like the number
   const uint32_t b = __float_as_uint(v);
@@ -44,30 +50,51 @@ __device__ __forceinline__ uint32_t ordered_bits(float v) {  // compares like th
 }
 __device__ __forceinline__ float from_ordered(uint32_t o) { return __uint_as_float((o & 0x80000000u) != 0 ? o ^ 0x80000000u : ~o); }
 
+__device__ __forceinline__ float just_below(float v) {  // -inf: -inf
+  return v == 0.f ? -1.401298464e-45f : v > -INFINITY ? from_ordered(ordered_bits(v) - 1) : v;
+}
+
 __device__ __forceinline__ double wave_sum_64(double v) {
 #pragma unroll
   for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, VELOX_WAVE);
   return v;
 }
 
-struct PieceSum { double sum; float top; int unused; };  // sum of exp(logit - top)
+struct PieceSum { double sum; float top; int unused; };  // sum of exp(logit - top); top: a number near the greatest logit
 struct Candidate { float logit; int token; };            // token < 0: none
 
-// Grid (pieces, rows).  sums: [row][piece]; candidates: [row][piece][keep], best first.
-template <int PER_THREAD>
-__global__ void __launch_bounds__(THREADS) beam_pieces_kernel(const float* __restrict__ logits, const float* __restrict__ scores, int vocab, int keep, int pieces,
-                                                              PieceSum* __restrict__ sums, Candidate* __restrict__ candidates) {
-  constexpr int PIECE = THREADS * PER_THREAD, QUADS = PER_THREAD / 4;
-  constexpr int PLACE_BITS = 13;
-  static_assert(PIECE <= 1 << PLACE_BITS, "a place of the piece fits its bits");
-  constexpr int MOST_LEFT = 32 * 4 * PER_THREAD;  // keys that may be left to rank: 32 parts of four threads, or 64 of one
-  __shared__ uint64_t left[MOST_LEFT];
-  __shared__ uint64_t part_best[THREADS];
-  __shared__ float wave_tops[THREADS / 64];
-  __shared__ double wave_sums[THREADS / 64];
-  __shared__ int num_left;
+constexpr int WAVES = THREADS / 64;
+constexpr int WAVE_LEFT = 512;  // a wave's list
 
-  const int row = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// The operation over the lanes of a row of 16, on every one of them.
+template <typename Op> __device__ __forceinline__ float over_row(float v, Op op) {
+#define VELOX_WITH(CONTROL) v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xf, 0xf, true)))
+  VELOX_WITH(0xB1);   // the neighbour,
+  VELOX_WITH(0x4E);   // the other two of four,
+  VELOX_WITH(0x141);  // the other four of eight,
+  VELOX_WITH(0x140);  // the other eight
+#undef VELOX_WITH
+  return v;
+}
+template <typename Op> __device__ __forceinline__ float over_wave(float v, Op op) {
+  v = over_row(v, op);
+  auto at = [&](int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); };
+  return op(op(at(0), at(16)), op(at(32), at(48)));
+}
+
+// Grid (pieces, rows); a piece is `span` tokens, a multiple of four, the row's last one may have fewer.  sums: [row][piece]; candidates:
+// [row][piece][keep], best first.  A round is UNITS loads of four tokens by every thread, the next one's in flight while one is worked.
+template <int UNITS>
+__global__ void __launch_bounds__(THREADS) beam_pieces_kernel(const float* __restrict__ logits, const float* __restrict__ scores, int vocab, int span, int keep, int pieces,
+                                                              PieceSum* __restrict__ sums, Candidate* __restrict__ candidates) {
+  constexpr int UNIT = 4 * THREADS, ROUND = UNITS * UNIT, PER_ROUND = 4 * UNITS;
+  __shared__ __attribute__((aligned(16))) uint64_t left[WAVES * WAVE_LEFT];
+  __shared__ double wave_sums[WAVES];
+  __shared__ float wave_refs[WAVES], wave_bounds[WAVES], wave_tops[WAVES];
+  __shared__ __attribute__((aligned(16))) float quarter_bounds[WAVES];
+  __shared__ int num_left[WAVES], reaches[2][WAVES];
+
+  const int row = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Candidate* const out = candidates + ((size_t)row * pieces + piece) * keep;
   if (!(scores[row] > -INFINITY)) {  // a beam that is not there: its continuations are all alike, the first tokens come first
     for (int r = tid; r < keep; r += THREADS) out[r] = Candidate{-INFINITY, piece == 0 && r < vocab ? r : -1};
@@ -77,99 +104,213 @@ __global__ void __launch_bounds__(THREADS) beam_pieces_kernel(const float* __res
   // (a row begins wherever the one before ends: loads of four numbers at any multiple of four bytes.  Which thread adds up which tokens
   // must not hang on that, or equal rows would differ in their sums' last bits)
   typedef float loose4_t __attribute__((ext_vector_type(4), aligned(4)));
-  const float* const first = logits + (size_t)row * vocab;
-  const int base = piece * PIECE;  // the piece's first token
-  float v[PER_THREAD];
+  const int base = piece * span, here = min(span, vocab - base);  // the piece's first token, its tokens
+  const float* const first = logits + (size_t)row * vocab + base;
+  auto load = [&](float (&v)[PER_ROUND], int round) {
 #pragma unroll
-  for (int q = 0; q < QUADS; ++q) {
-    const int token = base + 4 * (q * THREADS + tid);
-    if (token + 4 <= vocab) {
-      const loose4_t x = *reinterpret_cast<const loose4_t*>(first + token);
+    for (int q = 0; q < UNITS; ++q) {
+      const int start = round * ROUND + q * UNIT, place = start + 4 * tid;
+      if (start + UNIT <= here) {  // (the same for every thread)
+        const loose4_t x = *reinterpret_cast<const loose4_t*>(first + place);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * q + j] = x[j];
-    } else {
+        for (int j = 0; j < 4; ++j) v[4 * q + j] = x[j];
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * q + j] = token + j < vocab ? first[token + j] : -INFINITY;
-    }
-  }
-  if (tid == 0) num_left = 0;
-  float top = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < PER_THREAD; ++e) {
-    v[e] = v[e] == v[e] ? v[e] + 0.f : -INFINITY;  // (no number: never chosen before one; a zero has one form)
-    top = fmaxf(top, v[e]);
-  }
-  // keys: value, then place from the end; 0 for places outside the row
-  auto key_of = [&](int e) -> uint64_t {
-    const int place = 4 * ((e >> 2) * THREADS + tid) + (e & 3), token = base + place;
-    return token < vocab ? ((uint64_t)ordered_bits(v[e]) << PLACE_BITS) | (uint64_t)((1 << PLACE_BITS) - 1 - place) : 0;
-  };
-  uint64_t best = 0;
-#pragma unroll
-  for (int e = 0; e < PER_THREAD; ++e) {
-    const uint64_t k = key_of(e);
-    best = k > best ? k : best;
-  }
-  part_best[tid] = best;
-  const float wave_top = wave_max(top);
-  if (lane == 0) wave_tops[wave] = wave_top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) top = fmaxf(top, wave_tops[w]);
-  double sum = 0.0;
-  if (top > -INFINITY) {
-    const double ref = (double)top;
-#pragma unroll
-    for (int e = 0; e < PER_THREAD; ++e) sum += v[e] == top ? 1.0 : exp_below_zero(top < INFINITY ? (double)v[e] - ref : -INFINITY);
-  }
-  sum = wave_sum_64(sum);
-  if (lane == 0) wave_sums[wave] = sum;
-  // The bound: parts are single threads, or four of them while 64 parts are twice `keep`.  A wave finds the `keep`-th largest of the
-  // maxima bit by bit from the highest down; with fewer parts than `keep` that hold anything it is what all keys exceed.
-  uint64_t bound = 0;
-  {
-    uint64_t k[4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a) k[a] = part_best[64 * a + lane];
-    if (keep <= 32) {
-#pragma unroll
-      for (int a = 1; a < 4; ++a) {
-        k[0] = k[a] > k[0] ? k[a] : k[0];
-        k[a] = 0;
+        for (int j = 0; j < 4; ++j) v[4 * q + j] = place + j < here ? first[place + j] : -INFINITY;
       }
     }
-    for (int bit = 32 + PLACE_BITS - 1; bit >= 0; --bit) {
-      const uint64_t trial = bound | 1ull << bit;
-      int count = 0;
+  };
+  auto key_of = [&](float value, int place) -> uint64_t {  // (a zero has one form)
+    return (uint64_t)ordered_bits(value + 0.f) << 32 | (uint32_t)~place;
+  };
+  auto greatest = [](float a, float b) { return fmaxf(a, b); };
+  auto least = [](float a, float b) { return fminf(a, b); };
+
+  uint64_t* const list = left + wave * WAVE_LEFT;
+  int count = 0;
+  float mine = -INFINITY;          // the greatest that this lane has seen
+  float bound = -INFINITY;         // at least `keep` values of the rounds before are not below it
+  float ref = -INFINITY;           // what the sum's terms are relative to: any number that they do not exceed beyond 64 bits' range
+  double sum = 0.0;
+  auto cut = [&]() {  // the list's best `keep`
+    uint64_t k[WAVE_LEFT / 64], limit = 0;
 #pragma unroll
-      for (int a = 0; a < 4; ++a) count += __popcll(__ballot(k[a] >= trial));
-      if (count >= keep) bound = trial;
+    for (int a = 0; a < WAVE_LEFT / 64; ++a) k[a] = 64 * a + lane < count ? list[64 * a + lane] : 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t trial = limit | 1ull << bit;
+      int reach = 0;
+#pragma unroll
+      for (int a = 0; a < WAVE_LEFT / 64; ++a) reach += __popcll(__ballot(k[a] >= trial));
+      if (reach >= keep) limit = trial;
+    }
+    count = 0;
+#pragma unroll
+    for (int a = 0; a < WAVE_LEFT / 64; ++a) {
+      const uint64_t lanes = __ballot(k[a] >= limit);
+      if (k[a] >= limit) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = k[a];
+      count += __popcll(lanes);
+    }
+    return from_ordered((uint32_t)(limit >> 32));
+  };
+  float next_bound = -INFINITY;
+  auto take = [&](bool wanted, float value, int place) {
+    const uint64_t lanes = __ballot(wanted);
+    if (lanes == 0) return;
+    const int more = __popcll(lanes);
+    if (count + more > WAVE_LEFT) next_bound = fmaxf(next_bound, cut());
+    if (wanted) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = key_of(value, place);
+    count += more;
+  };
+  auto work = [&](const float (&v)[PER_ROUND], int round) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < PER_ROUND; ++e) most = fmaxf(most, v[e]);  // (what is no number is left out)
+    mine = fmaxf(mine, most);
+    auto with_lanes = [&](float part, int groups_from) {  // the least maximum of 64, 32, 16, 8 or 4 groups of lanes, at least as many as asked for
+      if (groups_from <= 32) part = fmaxf(part, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(part), 0xB1, 0xf, 0xf, true)));
+      if (groups_from <= 16) part = fmaxf(part, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(part), 0x4E, 0xf, 0xf, true)));
+      if (groups_from <= 8) part = fmaxf(part, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(part), 0x141, 0xf, 0xf, true)));
+      if (groups_from <= 4) part = fmaxf(part, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(part), 0x140, 0xf, 0xf, true)));
+      return over_wave(part, least);
+    };
+    next_bound = fmaxf(next_bound, with_lanes(mine, keep));
+    const float quarter = with_lanes(mine, (keep + 3) / 4);
+    volatile float* const published = quarter_bounds;
+    if (round == 0) {
+      if (lane == 0) published[wave] = quarter;
+      __syncthreads();
+    }
+    const float joint = fminf(fminf(published[0], published[1]), fminf(published[2], published[3]));
+    if (round > 0 && lane == 0) published[wave] = quarter;
+    const float above = fmaxf(round == 0 ? just_below(next_bound) : bound, just_below(joint));
+    const int at = round * ROUND + 4 * tid;
+    if (__ballot(most > above) != 0) {
+#pragma unroll
+      for (int e = 0; e < PER_ROUND; ++e) take(v[e] > above, v[e], at + (e >> 2) * UNIT + (e & 3));
+    }
+    if (round == 0 && wave == 0) {  // with fewer numbers than `keep` the first of the others fill up: they are among the first `keep` tokens
+#pragma unroll
+      for (int e = 0; e < 4; ++e) take(!(v[e] > -INFINITY) && 4 * tid + e < min(keep, here), -INFINITY, 4 * tid + e);
+    }
+    bound = next_bound;
+    if (__ballot(most > ref + 600.f) != 0) {  // the first numbers, or far beyond all before
+      const float now = over_wave(most, greatest);
+      sum = ref > -INFINITY && now < INFINITY && ref > now - FAR_BELOW ? sum * exp2_near_zero(((double)ref - (double)now) * LOG2_E) : 0.0;
+      ref = now;
+    }
+    if (ref == INFINITY) {
+#pragma unroll
+      for (int e = 0; e < PER_ROUND; ++e) sum += v[e] == INFINITY ? 1.0 : 0.0;
+    } else if (ref > -INFINITY) {
+      const double shift = -(double)ref * LOG2_E;
+      const float floor = ref - FAR_BELOW;
+      double second = 0.0;
+#pragma unroll
+      for (int e = 0; e < PER_ROUND; e += 2) {
+        sum += exp2_near_zero(fma((double)greater(floor, v[e]), LOG2_E, shift));
+        second += exp2_near_zero(fma((double)greater(floor, v[e + 1]), LOG2_E, shift));
+      }
+      sum += second;
+    }
+  };
+  {
+    float a[PER_ROUND], b[PER_ROUND];
+    const int rounds = (here + ROUND - 1) / ROUND;
+    load(a, 0);
+    for (int round = 0; round < rounds; round += 2) {
+      load(b, round + 1);  // (beyond the piece: nothing is loaded)
+      work(a, round);
+      if (round + 1 >= rounds) break;
+      load(a, round + 2);
+      work(b, round + 1);
     }
   }
-  bound = bound > 0 ? bound : 1;
-  __syncthreads();  // (num_left is set)
-#pragma unroll
-  for (int e = 0; e < PER_THREAD; ++e) {
-    const uint64_t k = key_of(e);
-    if (k >= bound) {
-      const int at = atomicAdd(&num_left, 1);
-      if (at < MOST_LEFT) left[at] = k;
-    }
+
+  // The waves' sums, and of their lists what reaches the greatest of their bounds.
+  sum = wave_sum_64(sum);
+  mine = over_wave(mine, greatest);
+  if (lane == 0) {
+    wave_tops[wave] = mine;
+    wave_sums[wave] = sum;
+    wave_refs[wave] = ref;
+    wave_bounds[wave] = bound;
   }
   __syncthreads();
-  const int count = min(num_left, MOST_LEFT);
-  for (int s = tid; s < count; s += THREADS) {
-    const uint64_t k = left[s];
-    int rank = 0;
-    for (int t = 0; t < count && rank < keep; ++t) rank += left[t] > k;
-    if (rank < keep) out[rank] = Candidate{from_ordered((uint32_t)(k >> PLACE_BITS)), base + (1 << PLACE_BITS) - 1 - (int)(k & ((1 << PLACE_BITS) - 1))};
-  }
-  for (int r = count + tid; r < keep; r += THREADS) out[r] = Candidate{-INFINITY, -1};
-  if (tid == 0) {
-    double total = 0.0;
+  float limit = -INFINITY, joint = INFINITY, top = -INFINITY, greatest_seen = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) total += wave_sums[w];
-    sums[(size_t)row * pieces + piece] = PieceSum{total, top, 0};
+  for (int w = 0; w < WAVES; ++w) {
+    limit = fmaxf(limit, wave_bounds[w]);
+    joint = fminf(joint, quarter_bounds[w]);
+    top = fmaxf(top, wave_refs[w]);
+    greatest_seen = fmaxf(greatest_seen, wave_tops[w]);
+  }
+  limit = fmaxf(limit, joint);
+  // That may be several times `keep`: a higher limit that `keep` or hardly more reach, by halving what lies between.
+  uint64_t k[WAVE_LEFT / 64];
+#pragma unroll
+  for (int a = 0; a < WAVE_LEFT / 64; ++a) k[a] = 64 * a + lane < count ? list[64 * a + lane] : 0;
+  int turn = 0;
+  auto reach_of = [&](uint32_t trial) {
+    int own = 0;
+#pragma unroll
+    for (int a = 0; a < WAVE_LEFT / 64; ++a) own += __popcll(__ballot((uint32_t)(k[a] >> 32) >= trial));
+    turn ^= 1;
+    if (lane == 0) reaches[turn][wave] = own;
+    __syncthreads();
+    return reaches[turn][0] + reaches[turn][1] + reaches[turn][2] + reaches[turn][3];
+  };
+  uint32_t lo = ordered_bits(limit + 0.f), hi = ordered_bits(greatest_seen) + 1;
+  for (int have = reach_of(lo); have > 2 * keep + 32 && hi - lo > 1;) {
+    const uint32_t trial = lo + (hi - lo) / 2;
+    const int reach = reach_of(trial);
+    if (reach >= keep) {
+      lo = trial;
+      have = reach;
+    } else {
+      hi = trial;
+    }
+  }
+  count = 0;
+#pragma unroll
+  for (int a = 0; a < WAVE_LEFT / 64; ++a) {
+    const bool stays = (uint32_t)(k[a] >> 32) >= lo;
+    const uint64_t lanes = __ballot(stays);
+    if (stays) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = k[a];
+    count += __popcll(lanes);
+  }
+  if (lane == 0) num_left[wave] = count;
+  __syncthreads();
+  // four threads to a value, each with one wave's list of the others
+  static_assert(WAVES == 4, "a list for each of the four");
+  const int counts[WAVES] = {num_left[0], num_left[1], num_left[2], num_left[3]};
+  const int total = counts[0] + counts[1] + counts[2] + counts[3];
+  const uint64_t* const others = left + (tid & 3) * WAVE_LEFT;
+  const int num_others = (tid & 3) == 0 ? counts[0] : (tid & 3) == 1 ? counts[1] : (tid & 3) == 2 ? counts[2] : counts[3];
+  for (int s = tid >> 2; s < total; s += THREADS / 4) {
+    int at = s, from = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES - 1; ++w) {
+      const bool behind = from == w && at >= counts[w];
+      at -= behind ? counts[w] : 0;
+      from += behind ? 1 : 0;
+    }
+    const uint64_t k = left[from * WAVE_LEFT + at];
+    int rank = 0;
+#pragma unroll 4
+    for (int t = 0; t < num_others; ++t) rank += others[t] > k;
+    rank += __shfl_xor(rank, 1, VELOX_WAVE);
+    rank += __shfl_xor(rank, 2, VELOX_WAVE);
+    if ((tid & 3) == 0 && rank < keep) out[rank] = Candidate{from_ordered((uint32_t)(k >> 32)), base + (int)~(uint32_t)k};
+  }
+  for (int r = total + tid; r < keep; r += THREADS) out[r] = Candidate{-INFINITY, -1};
+  if (tid == 0) {
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float own = wave_refs[w];
+      if (own > -INFINITY) all += own == top ? wave_sums[w] : top < INFINITY ? wave_sums[w] * exp2_near_zero(((double)fmaxf(own, top - FAR_BELOW) - (double)top) * LOG2_E) : 0.0;
+    }
+    sums[(size_t)row * pieces + piece] = PieceSum{all, top, 0};
   }
 }
 
@@ -182,89 +323,174 @@ __device__ __forceinline__ uint64_t after_of(int beam, float logit, int token) {
 __device__ __forceinline__ bool before(const Place& a, const Place& b) { return a.value > b.value || (a.value == b.value && a.after < b.after); }
 constexpr int MOST_BEAMS = 256, MOST_VOCAB = 1 << 24;
 
-// Grid (requests).  A list is a piece's candidates in order, `beams * pieces` of them.  Of the lists' first ones the `keep`-th best is a
-// bound: no list whose first lies behind it holds anything that is wanted, and at most `keep` lists do not.
+// Grid (requests).  All candidates' values are worked out, and the `keep` best found by counting: a bound that at least `keep` and hardly
+// more candidates reach is looked for from the best value down in steps that double, then by halving the interval that is left, as a
+// number whose order is the values' (64 bits), and should too many have the very same value, among those by what else decides.  What the
+// bound leaves is ranked.  (Bounds from the lists' first entries alone leave nearly everything where the beams' scores lie far apart.)
 constexpr int JOIN_THREADS = 1024;
-constexpr int JOIN_LEFT = MOST_KEPT * MOST_KEPT;
+constexpr int JOIN_WAVES = JOIN_THREADS / 64;
+constexpr int JOIN_HELD = 4;   // candidates a thread keeps in registers; the others' values lie in memory
+constexpr int JOIN_LEFT = 2 * MOST_KEPT + 64;
+
+__device__ __forceinline__ uint64_t ordered_bits_64(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+  return b ^ ((uint64_t)((long long)b >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double from_ordered_64(uint64_t o) { return __longlong_as_double((long long)((o >> 63) != 0 ? o ^ 0x8000000000000000ull : ~o)); }
+
 __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const float* __restrict__ scores, const PieceSum* __restrict__ sums, const Candidate* __restrict__ candidates,
-                                                                 int beams, int keep, int pieces, float* __restrict__ out_scores, int* __restrict__ out_parents,
-                                                                 int* __restrict__ out_tokens) {
-  __shared__ Place left[JOIN_LEFT];  // (the lists' firsts before)
+                                                                 int beams, int keep, int pieces, uint64_t* __restrict__ values, float* __restrict__ out_scores,
+                                                                 int* __restrict__ out_parents, int* __restrict__ out_tokens) {
+  __shared__ Place left[JOIN_LEFT];
   __shared__ double offsets[MOST_BEAMS], tops[MOST_BEAMS];
-  __shared__ Place limit;
+  __shared__ float beam_scores[MOST_BEAMS];
+  __shared__ __attribute__((aligned(16))) int counts[2][JOIN_WAVES];
+  __shared__ uint64_t wave_best[JOIN_WAVES];
   __shared__ int num_left;
   const int request = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t row0 = (size_t)request * beams;
-  const int lists = beams * pieces;
-  const Place last = {-INFINITY, ~0ull};
+  const int per_beam = pieces * keep, total = beams * per_beam;  // (below 2^31: the launcher sees to it)
+  const Candidate* const mine = candidates + row0 * per_beam;
+  uint64_t* const rest = values + row0 * per_beam;
+  // (asked for before the sums: they are on nobody's way)
+  Candidate held[JOIN_HELD];
+#pragma unroll
+  for (int k = 0; k < JOIN_HELD; ++k) {
+    const int at = tid + k * JOIN_THREADS;
+    held[k] = at < total ? mine[at] : Candidate{-INFINITY, -1};
+  }
   // a beam's maximum, and minus the logarithm of its sum
-  for (int w = wave; w < beams; w += JOIN_THREADS / 64) {
+  for (int w = wave; w < beams; w += JOIN_WAVES) {
     const PieceSum* s = sums + (row0 + w) * pieces;
-    float top = -INFINITY;
-    for (int p = lane; p < pieces; p += 64) top = fmaxf(top, s[p].top);
+    const PieceSum own = lane < pieces ? s[lane] : PieceSum{0.0, -INFINITY, 0};
+    float top = own.top;
+    for (int p = 64 + lane; p < pieces; p += 64) top = fmaxf(top, s[p].top);
     top = wave_max(top);
-    double sum = 0.0;
-    for (int p = lane; p < pieces; p += 64) {
-      const PieceSum x = s[p];
-      if (x.top > -INFINITY) sum += x.top == top ? x.sum : x.sum * exp_below_zero(top < INFINITY ? (double)x.top - (double)top : -INFINITY);
-    }
+    auto part = [&](const PieceSum& x) {
+      return x.top > -INFINITY ? (x.top == top ? x.sum : top < INFINITY ? x.sum * exp2_near_zero(((double)fmaxf(x.top, top - FAR_BELOW) - (double)top) * LOG2_E) : 0.0) : 0.0;
+    };
+    double sum = part(own);
+    for (int p = 64 + lane; p < pieces; p += 64) sum += part(s[p]);
     sum = wave_sum_64(sum);
     if (lane == 0) {
       tops[w] = (double)top;
       offsets[w] = top > -INFINITY ? -log(sum) : 0.0;
+      beam_scores[w] = scores[row0 + w];
     }
   }
-  if (tid == 0) {
-    num_left = 0;
-    limit = last;
-  }
+  if (tid == 0) num_left = 0;
   __syncthreads();
-  const Candidate* const mine = candidates + row0 * pieces * keep;
-  auto place_of = [&](int w, const Candidate& c) -> Place {
-    const float score = scores[row0 + w];
-    const double top = tops[w];
-    const double value = !(c.logit > -INFINITY) || !(score > -INFINITY) ? -INFINITY : (double)score + (((double)c.logit == top ? 0.0 : (double)c.logit - top) + offsets[w]);
-    return Place{value, after_of(w, c.logit, c.token)};
+  auto beam_of = [&](int at) { return (int)((unsigned)at / (unsigned)per_beam); };
+  auto key_of = [&](int at, const Candidate& c) -> uint64_t {  // 0: no candidate
+    if (c.token < 0) return 0;
+    const int w = beam_of(at);
+    const double score = (double)beam_scores[w], top = tops[w];
+    return ordered_bits_64(!(c.logit > -INFINITY) || !(score > -INFINITY) ? -INFINITY : score + (((double)c.logit == top ? 0.0 : (double)c.logit - top) + offsets[w]));
   };
-  auto first_of = [&](int a) -> Place {
-    if (a >= lists) return last;
-    const Candidate c = mine[(size_t)a * keep];
-    return c.token >= 0 ? place_of(a / pieces, c) : last;
+  uint64_t key[JOIN_HELD], best = 0;
+#pragma unroll
+  for (int k = 0; k < JOIN_HELD; ++k) {
+    key[k] = key_of(tid + k * JOIN_THREADS, held[k]);
+    best = key[k] > best ? key[k] : best;
+  }
+  for (int at = tid + JOIN_HELD * JOIN_THREADS; at < total; at += JOIN_THREADS) {
+    const uint64_t k = key_of(at, mine[at]);
+    rest[at] = k;  // (read again by this thread alone)
+    best = k > best ? k : best;
+  }
+#pragma unroll
+  for (int offset = 1; offset < 64; offset <<= 1) {
+    const uint64_t other = (uint64_t)__shfl_xor((unsigned long long)best, offset, VELOX_WAVE);
+    best = other > best ? other : best;
+  }
+  if (lane == 0) wave_best[wave] = best;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < JOIN_WAVES; ++w) best = wave_best[w] > best ? wave_best[w] : best;
+
+  int turn = 0;
+  auto count_of = [&](auto reaches) -> int {  // reaches(key, place among the candidates)
+    int own = 0;
+#pragma unroll
+    for (int k = 0; k < JOIN_HELD; ++k) own += __popcll(__ballot(reaches(key[k], tid + k * JOIN_THREADS)));
+    for (int base = JOIN_HELD * JOIN_THREADS; base < total; base += JOIN_THREADS) {
+      const int at = base + tid;
+      own += __popcll(__ballot(at < total && reaches(rest[at < total ? at : total - 1], at)));
+    }
+    turn ^= 1;
+    if (lane == 0) counts[turn][wave] = own;
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < JOIN_WAVES; ++w) sum += counts[turn][w];
+    return sum;
   };
-  if (lists >= keep) {
-    for (int a0 = 0; a0 < lists; a0 += JOIN_THREADS) {
-      const Place own = first_of(a0 + tid);
-      int rank = 0;
-      for (int o0 = 0; o0 < lists; o0 += JOIN_THREADS) {
-        __syncthreads();
-        left[tid] = o0 == a0 ? own : first_of(o0 + tid);
-        __syncthreads();
-        const int here = min(lists - o0, JOIN_THREADS);
-        for (int o = 0; o < here; ++o) rank += before(left[o], own);
+  // at least `keep` candidates have lo, fewer have hi; of a value of -inf and of places without a candidate: lo = 1 is what all have
+  const int most = 2 * keep + 16;
+  uint64_t lo = 1, hi = best + 1;
+  int have = total;
+  const double top_value = from_ordered_64(best);
+  if (top_value > -INFINITY && top_value < INFINITY) {
+    for (double below = 2.0; below <= 1024.0; below *= 2.0) {
+      const uint64_t trial = ordered_bits_64(top_value - below);
+      const int count = count_of([&](uint64_t k, int) { return k >= trial; });
+      if (count >= keep) {
+        lo = trial;
+        have = count;
+        break;
       }
-      if (rank == keep - 1 && own.after != last.after) limit = own;
+      hi = trial;
     }
   }
-  __syncthreads();
-  const Place bound = limit;
-  for (int a = tid; a < lists; a += JOIN_THREADS) {
-    const int w = a / pieces;
-    for (int r = 0; r < keep; ++r) {
-      const Candidate c = mine[(size_t)a * keep + r];
-      if (c.token < 0) break;
-      const Place place = place_of(w, c);
-      if (before(bound, place)) break;  // (the list is in order)
-      const int at = atomicAdd(&num_left, 1);
-      if (at < JOIN_LEFT) left[at] = place;
+  while (have > most && hi - lo > 1) {
+    const uint64_t trial = lo + (hi - lo) / 2;
+    const int count = count_of([&](uint64_t k, int) { return k >= trial; });
+    if (count >= keep) {
+      lo = trial;
+      have = count;
+    } else {
+      hi = trial;
     }
   }
+  // of those with the value lo itself only the ones up to `until` (by after_of)
+  auto after_at = [&](int at) { const Candidate c = mine[at]; return after_of(beam_of(at), c.logit, c.token); };
+  uint64_t until = ~0ull;
+  if (have > most) {
+    const int above = count_of([&](uint64_t k, int) { return k > lo; });
+    uint64_t from = 0;  // fewer than are missing lie before or at it, or none
+    while (have > most && until - from > 1) {
+      const uint64_t trial = from + (until - from) / 2;
+      const int count = above + count_of([&](uint64_t k, int at) { return k == lo && after_at(at) <= trial; });
+      if (count >= keep) {
+        until = trial;
+        have = count;
+      } else {
+        from = trial;
+      }
+    }
+  }
+  auto offer = [&](uint64_t k, int at) {
+    if (k < lo) return;
+    const uint64_t after = after_at(at);
+    if (k == lo && after > until) return;
+    const int to = atomicAdd(&num_left, 1);
+    if (to < JOIN_LEFT) left[to] = Place{from_ordered_64(k), after};
+  };
+#pragma unroll
+  for (int k = 0; k < JOIN_HELD; ++k) offer(key[k], tid + k * JOIN_THREADS);
+  for (int at = tid + JOIN_HELD * JOIN_THREADS; at < total; at += JOIN_THREADS) offer(rest[at], at);
   __syncthreads();
+  // eight threads to a place, each with an eighth of the others
   const int count = min(num_left, JOIN_LEFT);
-  for (int s = tid; s < count; s += JOIN_THREADS) {
+  for (int s = tid >> 3; s < count; s += JOIN_THREADS / 8) {
     const Place place = left[s];
     int rank = 0;
-    for (int t = 0; t < count && rank < keep; ++t) rank += before(left[t], place);
-    if (rank >= keep) continue;
+#pragma unroll 4
+    for (int t = tid & 7; t < count; t += 8) rank += before(left[t], place);
+    rank += __shfl_xor(rank, 1, VELOX_WAVE);
+    rank += __shfl_xor(rank, 2, VELOX_WAVE);
+    rank += __shfl_xor(rank, 4, VELOX_WAVE);
+    if ((tid & 7) != 0 || rank >= keep) continue;
     const size_t at = (size_t)request * keep + rank;
     out_scores[at] = (float)place.value;
     out_parents[at] = (int)(place.after >> 56);
@@ -275,27 +501,26 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const float* __
 extern "C" int velox_beam_most_kept() { return MOST_KEPT; }
 extern "C" int velox_beam_most_beams() { return MOST_BEAMS; }
 extern "C" int velox_beam_most_vocab() { return MOST_VOCAB; }
-// pieces of a row; `per_thread` is 8 or 32
-extern "C" int velox_beam_pieces(int vocab, int per_thread) { return (vocab + THREADS * per_thread - 1) / (THREADS * per_thread); }
 extern "C" long long velox_beam_scratch_bytes(int rows, int pieces, int keep) {
-  return (long long)rows * pieces * ((long long)sizeof(PieceSum) + (long long)keep * sizeof(Candidate));
+  return (long long)rows * pieces * ((long long)sizeof(PieceSum) + (long long)keep * (sizeof(uint64_t) + sizeof(Candidate)));
 }
-extern "C" int velox_beam_select(const float* logits, const float* scores, int requests, int beams, int vocab, int keep, int per_thread, void* scratch,
+extern "C" int velox_beam_select(const float* logits, const float* scores, int requests, int beams, int vocab, int keep, int pieces, void* scratch,
                                  long long scratch_bytes, float* out_scores, int* out_parents, int* out_tokens, hipStream_t stream) {
   if (requests <= 0) return 0;
-  const int pieces = velox_beam_pieces(vocab, per_thread);
   const long long rows = (long long)requests * beams;
-  if (beams < 1 || beams > MOST_BEAMS || vocab < 1 || vocab > MOST_VOCAB || keep < 1 || keep > MOST_KEPT || (per_thread != 8 && per_thread != 32)) return -1;
-  if (rows > 65535 || keep > (long long)beams * vocab) return -1;
+  if (beams < 1 || beams > MOST_BEAMS || vocab < 1 || vocab > MOST_VOCAB || keep < 1 || keep > MOST_KEPT || pieces < 1) return -1;
+  if (rows > 65535 || keep > (long long)beams * vocab || (long long)beams * pieces * keep > 0x7fff0000LL) return -1;
   if (scratch_bytes < velox_beam_scratch_bytes((int)rows, pieces, keep)) return -1;
   PieceSum* const sums = (PieceSum*)scratch;
-  Candidate* const candidates = (Candidate*)(sums + rows * pieces);
+  uint64_t* const values = (uint64_t*)(sums + rows * pieces);
+  Candidate* const candidates = (Candidate*)(values + rows * pieces * keep);
   const dim3 grid(pieces, (unsigned)rows);
-  if (per_thread == 8) beam_pieces_kernel<8><<<grid, THREADS, 0, stream>>>(logits, scores, vocab, keep, pieces, sums, candidates);
-  else beam_pieces_kernel<32><<<grid, THREADS, 0, stream>>>(logits, scores, vocab, keep, pieces, sums, candidates);
+  const int span = ((vocab + pieces - 1) / pieces + 3) / 4 * 4;  // (the last ones may be short, or have nothing)
+  if (span <= 2 * 4 * THREADS) beam_pieces_kernel<2><<<grid, THREADS, 0, stream>>>(logits, scores, vocab, span, keep, pieces, sums, candidates);
+  else beam_pieces_kernel<4><<<grid, THREADS, 0, stream>>>(logits, scores, vocab, span, keep, pieces, sums, candidates);
   const int status = (int)hipGetLastError();
   if (status != 0) return status;
-  beam_join_kernel<<<requests, JOIN_THREADS, 0, stream>>>(scores, sums, candidates, beams, keep, pieces, out_scores, out_parents, out_tokens);
+  beam_join_kernel<<<requests, JOIN_THREADS, 0, stream>>>(scores, sums, candidates, beams, keep, pieces, values, out_scores, out_parents, out_tokens);
   return (int)hipGetLastError();
 }
 

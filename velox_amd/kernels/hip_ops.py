@@ -289,12 +289,11 @@ class HipOps:
         """The kernels of ``beam_select`` and ``reorder_states``."""
         if self._beams is None:
             lib = ctypes.CDLL(build.ensure_beams())
-            lib.velox_beam_pieces.argtypes = [_I, _I]
             lib.velox_beam_scratch_bytes.argtypes = [_I, _I, _I]
             lib.velox_beam_scratch_bytes.restype = ctypes.c_longlong
             lib.velox_beam_select.argtypes = [_P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _P, _P, _P]
             lib.velox_reorder_states.argtypes = [_P, _I, _P, _P, _I, _I, _I, _P]
-            for fn in (lib.velox_beam_pieces, lib.velox_beam_select, lib.velox_reorder_states):
+            for fn in (lib.velox_beam_select, lib.velox_reorder_states):
                 fn.restype = _I
             self._beams = lib
         return self._beams
@@ -2388,6 +2387,12 @@ class HipOps:
         self._launched(status, "shared_prefix_attention")
         return out
 
+    def _beam_pieces(self, rows: int, vocab: int) -> int:
+        """Into how many pieces ``beam_select`` cuts a row: as many as give the compute units two and a half workgroups each, of 2,048 tokens at least.
+        Measured on MI355X (us, the kernel that reads the logits): 512 rows of 152,064 whole 100, in 2 pieces 83, in 4 86; 64 rows in 4 25.0, in 8
+        19.7, in 16 21.1; 168 rows of 32,003 in 2 19.7, in 4 16.8, in 8 20.5."""
+        return max(1, min(-(-5 * self.num_cus // (2 * rows)), -(-vocab // 2048)))
+
     def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, keep: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """The ``keep`` best continuations of every request over its beams and the vocabulary.  ``logits`` float32 ``[requests * beams, vocab]``,
         ``scores`` float32 ``[requests, beams]``, the beams' sums of log-probabilities (-inf: a beam that is not there).  A continuation of beam ``w``
@@ -2412,11 +2417,11 @@ class HipOps:
         if requests == 0:
             return values, parents, tokens
         lib = self.beam_library()
-        per_thread = 32 if rows * lib.velox_beam_pieces(vocab, 32) >= 2 * self.num_cus else 8
-        size = int(lib.velox_beam_scratch_bytes(rows, lib.velox_beam_pieces(vocab, per_thread), keep))
+        pieces = self._beam_pieces(rows, vocab)
+        size = int(lib.velox_beam_scratch_bytes(rows, pieces, keep))
         scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
         with self._current():
-            status = lib.velox_beam_select(_ptr(logits), _ptr(scores), requests, beams, vocab, keep, per_thread, _ptr(scratch), size, _ptr(values), _ptr(parents), _ptr(tokens),
+            status = lib.velox_beam_select(_ptr(logits), _ptr(scores), requests, beams, vocab, keep, pieces, _ptr(scratch), size, _ptr(values), _ptr(parents), _ptr(tokens),
                                            self._stream())
         self._launched(status, "beam_select")
         return values, parents, tokens
