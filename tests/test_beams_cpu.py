@@ -89,19 +89,24 @@ def test_attention_items_are_enough(ops, heads, kv_heads, dim):
     for _ in range(300):
         sizes = [rng.choice([0, 1, 2, 3, 17, 70]) for _ in range(rng.randint(0, 9))]
         num_seqs = max(1, sum(sizes) + rng.randint(0, 5))
-        row_tiles, target, items = ops._shared_prefix_shape(num_seqs, len(sizes), heads, kv_heads, dim, rng.choice([2, 4]), max(sizes + [1]))
-        steps = lambda low, high: -(-(high - low // 32 * 32) // 128) if high > low else 0  # noqa: E731
-        work = []  # (row blocks, steps)
-        b = 0
+        element_size = rng.choice([2, 4])
+        tile = 32 if element_size == 2 else 16
+        row_tiles, target, items, rows = ops._shared_prefix_shape(num_seqs, len(sizes), heads, kv_heads, dim, element_size, max(sizes + [1]))
+        own_blocks = -(-group // 16)
+        shared_work, own_work = [], []  # (row blocks, steps) of the groups, tiles of the sequences
         for size in sizes:
             shared = rng.choice([0, 1, 5, 128, 1000, 33333]) if size > 1 else 0
             if shared:
-                work.append((-(-size * group // (16 * row_tiles)), steps(0, shared)))
-            work += [(-(-group // 16), steps(shared, shared + rng.choice([0, 1, 200, 5000]))) for _ in range(size)]
-            b += size
-        work += [(-(-group // 16), steps(0, rng.choice([0, 1, 200, 5000]))) for _ in range(num_seqs - b)]
-        per = max(1, -(-sum(x * y for x, y in work) // target))
-        assert sum(x * -(-y // per) for x, y in work) <= items
+                shared_work.append((-(-size * group // (16 * row_tiles)), -(-shared // (4 * tile))))
+            for _ in range(size):
+                more = rng.choice([0, 1, 200, 5000])
+                own_work.append(-(-(shared + more - shared // tile * tile) // tile) if more else 0)
+        own_work += [-(-rng.choice([0, 1, 200, 5000]) // tile) for _ in range(num_seqs - len(own_work))]
+        per = max(1, -(-(sum(x * y for x, y in shared_work) + -(-own_blocks * sum(own_work) // 4)) // target))
+        shared_items = sum(x * -(-y // per) for x, y in shared_work)
+        own_items = sum(own_blocks * max(1, -(-y // per)) for y in own_work)
+        assert shared_items + -(-own_items // 4) <= items
+        assert shared_items * 16 * row_tiles + own_items * 16 <= rows
 
 
 @pytest.mark.parametrize("logits,scores,keep,says", [

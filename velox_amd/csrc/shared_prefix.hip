@@ -10,10 +10,11 @@
 // are the same for the group's sequences, so n_g G rows of queries stand against one stream of keys and values, which is read
 // once; the second part is each sequence's own, G rows against its keys.
 //
-// Both parts are cut into items of about equally many keys (see `Plan`), one workgroup each and all in one launch; a second
-// kernel joins what the items leave.  A workgroup's four waves take 32 keys in turn, each straight from the cache into the
-// operands of matrix instructions, the next tile in flight while one is multiplied: no wave shares a key with another, so
-// nothing is staged and no barrier stands in the loop.  Rows are held as tiles of 16, RT of them in every wave.
+// Both parts are cut into items of about equally many keys (see `Plan`), all in one launch; a second kernel joins what the items leave.
+// A group's item is a workgroup's: its four waves take a tile of keys in turn, each straight from the cache into the operands of matrix
+// instructions, and put their results together at the end.  A sequence's own keys are single waves' items, four of them to a workgroup.  No
+// wave shares a key with another, so nothing is staged and no barrier stands in the loop: the next tile's keys are asked for as soon as
+// this one's have been multiplied, its values as soon as this one's have, two workgroups to a compute unit.
 //
 // Matrix cores: S^T[key, row] = K Q^T and O^T[channel, row] = V^T P^T, both with 16 x 16 results.  For a block of KB contraction
 // indices (32 in bfloat16, 16 in float32) lane (g = lane / 16, i = lane % 16) holds 16 bytes of row or column i, those of place g; a result is rows
@@ -27,16 +28,14 @@
 constexpr int D = VELOX_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head size must be a multiple of 16 between 16 and 256");
 
-constexpr int TILE = 32;                 // keys a wave takes at a time
-constexpr int WAVES = 4;
-constexpr int STEP = TILE * WAVES;       // keys a workgroup takes at a time
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
 constexpr int MOST_GROUPS = 1024;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 template <typename T> struct Block;
 template <> struct Block<bf16_t> {
-  static constexpr int KB = 32, VEC = 8;
+  static constexpr int KB = 32, VEC = 8;  // a tile of keys is one block of the second product: KB keys, KB / 16 score tiles
   static constexpr float SCALE = 1.44269504088896340736f, LN_UNIT = 0.69314718055994530942f;  // scores in powers of two
   static __device__ __forceinline__ float4_t mma(const float4_t& a, const float4_t& b, const float4_t& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -72,121 +71,169 @@ template <> struct Block<float> {
 // ---- which workgroup does what -----------------------------------------------------------------------------------------
 // Everything is worked out from the lengths on the device, so that a captured step replays with other lengths.  A group's shared
 // keys are those of its first sequence at most (it is through that one's table that they are read); a sequence with fewer keys
-// than its group shares, and one that is alone in its group or in none, shares nothing.  The steps of STEP keys of all items
-// together over `target` workgroups are what one item may have; a group's rows are cut into blocks of `block_rows`, a
-// sequence's G rows into blocks of 16.
+// than its group shares, and one that is alone in its group or in none, shares nothing.  A step is a tile of keys for each of four waves; all
+// items' steps over `target` workgroups are what one item may have (`per`: of a sequence's own keys, tiles of one wave).  A group's rows are cut
+// into blocks of `block_rows`, a sequence's G rows into blocks of 16.
+//
+// What the items leave has rows of its own, per KV head: `block_rows` for every item of a group, in the order groups, parts of the keys, row blocks, then
+// 16 for every item of a sequence, in the order sequences, parts, blocks.  Row r of a group's or of a sequence's part p then lies at
+// start + p stride + r.
 struct Lengths {
   const int* kv_lens;
   const int* group_starts;
   const int* shared_lens;
   int num_seqs, num_groups, group, block_rows, target;  // group: query heads of a KV head
   int most;                                             // keys a table has room for
+  int rows_room;
 };
 
-struct Groups {  // in LDS
+constexpr int LENS_HELD = 1024;
+struct Plan {  // in LDS
   int start[MOST_GROUPS], end[MOST_GROUPS], shared[MOST_GROUPS];
+  int before[MOST_GROUPS];  // items of the groups before
+  int lens[LENS_HELD];
+};
+struct Directory { int shared_at, shared_stride, shared_parts, own_at, own_parts, unused[3]; };  // of a sequence: where its rows lie
+struct Item {           // group >= 0: of that group's shared keys, by the whole workgroup; else sequence >= 0: of its own keys, by this wave; else none
+  int group, sequence;
+  int first, count;     // the group's first sequence, and how many it has
+  int block, from, to;  // row block, keys
+  int at;               // its rows' place
+  bool tells;           // it writes the directory
+  Directory rows;
 };
 
 __device__ __forceinline__ int clamped(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
-
-__device__ __forceinline__ int keys_of(const Lengths& l, int b) { return clamped(l.kv_lens[b], 0, l.most); }
-
-__device__ __forceinline__ void load_groups(const Lengths& l, Groups& groups) {
-  for (int g = threadIdx.x; g < l.num_groups; g += blockDim.x) {
-    const int start = clamped(l.group_starts[g], 0, l.num_seqs), end = clamped(l.group_starts[g + 1], start, l.num_seqs);
-    groups.start[g] = start;
-    groups.end[g] = end;
-    groups.shared[g] = end - start > 1 ? clamped(l.shared_lens[g], 0, keys_of(l, start)) : 0;
-  }
-  __syncthreads();
+// a / b rounded down, 0 <= a < 2^23 <= 2^31 / b: by the reciprocal, which is off by one at most
+__device__ __forceinline__ int quotient(int a, int b) {
+  int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+  const int rest = a - q * b;
+  q += rest >= b ? 1 : 0;
+  q -= rest < 0 ? 1 : 0;
+  return q;
 }
+__device__ __forceinline__ int parts_of(int steps, int per) { return quotient(steps + per - 1, per); }
 
-struct Own { int group, from, to; };  // a sequence's own keys [from, to); group: whose shared keys it has, or -1
-__device__ __forceinline__ Own own_of(const Lengths& l, const Groups& groups, int b) {
-  const int len = keys_of(l, b);
-  int lo = -1, hi = l.num_groups;  // the last group that begins at b or before
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (groups.start[mid] <= b) lo = mid;
-    else hi = mid;
-  }
-  const bool shares = lo >= 0 && b < groups.end[lo < 0 ? 0 : lo] && groups.shared[lo < 0 ? 0 : lo] > 0 && groups.shared[lo < 0 ? 0 : lo] <= len;
-  return Own{shares ? lo : -1, shares ? groups.shared[lo] : 0, len};
-}
-__device__ __forceinline__ int steps_between(int from, int to) { return to > from ? (to - from / TILE * TILE + STEP - 1) / STEP : 0; }
-
-__device__ __forceinline__ int wave_add(int v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, VELOX_WAVE);
-  return v;
-}
-__device__ __forceinline__ int wave_add_up_to(int v) {  // v plus those of the lanes before
-#pragma unroll
-  for (int offset = 1; offset < 64; offset <<= 1) {
-    const int w = __shfl_up(v, offset, VELOX_WAVE);
-    if ((int)(threadIdx.x & 63) >= offset) v += w;
-  }
+// v plus those of the lanes before
+__device__ __forceinline__ int sum_up_to_lane(int v) {
+#define VELOX_ADD_SHIFTED(CONTROL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false)
+  VELOX_ADD_SHIFTED(0x111, 0xf);  // from 1, 2, 4 and 8 lanes down in a row of 16,
+  VELOX_ADD_SHIFTED(0x112, 0xf);
+  VELOX_ADD_SHIFTED(0x114, 0xf);
+  VELOX_ADD_SHIFTED(0x118, 0xf);
+  VELOX_ADD_SHIFTED(0x142, 0xa);  // from the end of the row before, into the second and the fourth,
+  VELOX_ADD_SHIFTED(0x143, 0xc);  // from the middle, into the upper half
+#undef VELOX_ADD_SHIFTED
   return v;
 }
 
-__device__ __forceinline__ int blocks_of(const Lengths& l, const Groups& groups, int g) {
-  return groups.shared[g] > 0 ? ((groups.end[g] - groups.start[g]) * l.group + l.block_rows - 1) / l.block_rows : 0;
-}
-
-// steps of one item (the whole wave takes part)
-__device__ __forceinline__ int steps_per_item(const Lengths& l, const Groups& groups) {
-  const int lane = threadIdx.x & 63, own_blocks = (l.group + 15) / 16;
-  int total = 0;
-  for (int g = lane; g < l.num_groups; g += 64) total += blocks_of(l, groups, g) * steps_between(0, groups.shared[g]);
-  for (int b = lane; b < l.num_seqs; b += 64) {
-    const Own own = own_of(l, groups, b);
-    total += own_blocks * steps_between(own.from, own.to);
+// The item of workgroup `wg`, and in it of this wave.  Every wave works it out for itself (all write the same to `plan`, and each reads what
+// it has written), with no barrier: a lane has a group and a sequence of its own, 64 of each at a time.
+template <int TILE>
+__device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) {
+  constexpr int STEP = WAVES * TILE;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int own_blocks = (l.group + 15) / 16, block_shift = 31 - __builtin_clz(l.block_rows);
+  auto at_most = [](int v, int count) { return v < count ? v : count - 1; };
+  // (everything that a lane's first group and sequence need is asked for before any of it is waited for)
+  int start0 = 0, end0 = 0, shared0 = 0;
+  if (l.num_groups > 0) {
+    const int g = at_most(lane, l.num_groups);
+    start0 = l.group_starts[g];
+    end0 = l.group_starts[g + 1];
+    shared0 = l.shared_lens[g];
   }
-  total = wave_add(total);
-  return max(1, (total + l.target - 1) / l.target);
-}
-
-// Items in their order: group by group, of each the parts of the keys, of each part the row blocks; then sequence by sequence the
-// same.  `before` of either: the items before it.
-struct Item { int group, sequence, block, part, per; };  // group >= 0: of a group's shared keys; else sequence >= 0; else none
-
-__device__ __forceinline__ Item find_item(const Lengths& l, const Groups& groups, int item) {
-  const int lane = threadIdx.x & 63, own_blocks = (l.group + 15) / 16;
-  const int per = steps_per_item(l, groups);
+  const int len0 = l.kv_lens[at_most(lane, l.num_seqs)];
+  for (int b = lane; b < l.num_seqs && b < LENS_HELD; b += 64) plan.lens[b] = clamped(b < 64 ? len0 : l.kv_lens[b], 0, l.most);
+  auto keys_of = [&](int b) { return b < LENS_HELD ? plan.lens[b] : clamped(l.kv_lens[b], 0, l.most); };
+  for (int g = lane; g < l.num_groups; g += 64) {
+    const int start = clamped(g < 64 ? start0 : l.group_starts[g], 0, l.num_seqs), end = clamped(g < 64 ? end0 : l.group_starts[g + 1], start, l.num_seqs);
+    plan.start[g] = start;
+    plan.end[g] = end;
+    plan.shared[g] = end - start > 1 ? clamped(g < 64 ? shared0 : l.shared_lens[g], 0, keys_of(start)) : 0;
+  }
+  struct Own { int group, from, to; };  // a sequence's own keys [from, to); group: whose shared keys it has, or -1
+  auto own_of = [&](int b) {
+    const int len = keys_of(b);
+    int lo = -1, hi = l.num_groups;  // the last group that begins at b or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (plan.start[mid] <= b) lo = mid;
+      else hi = mid;
+    }
+    const int shared = lo >= 0 && b < plan.end[lo] ? plan.shared[lo] : 0;
+    return shared > 0 && shared <= len ? Own{lo, shared, len} : Own{-1, 0, len};
+  };
+  auto blocks_of = [&](int g) { return plan.shared[g] > 0 ? ((plan.end[g] - plan.start[g]) * l.group + l.block_rows - 1) >> block_shift : 0; };
+  auto steps_of = [&](int keys) { return (unsigned)(keys + STEP - 1) / STEP; };
+  auto tiles_of = [&](const Own& own) { return own.to > own.from ? (int)((unsigned)(own.to + TILE - 1) / TILE - (unsigned)own.from / TILE) : 0; };
+  // steps of all items, and how many one may have
+  const Own own0 = lane < l.num_seqs ? own_of(lane) : Own{-1, 0, 0};
+  int steps = 0, tiles = lane < l.num_seqs ? own_blocks * tiles_of(own0) : 0;
+  for (int g = lane; g < l.num_groups; g += 64) steps += blocks_of(g) * steps_of(plan.shared[g]);
+  for (int b = 64 + lane; b < l.num_seqs; b += 64) tiles += own_blocks * tiles_of(own_of(b));
+  steps = __builtin_amdgcn_readlane(sum_up_to_lane(steps), 63);
+  tiles = __builtin_amdgcn_readlane(sum_up_to_lane(tiles), 63);
+  const int per = max(1, (steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target);
+  // the groups' items
+  Item found = {-1, -1, 0, 0, 0, 0, 0, 0, false, {}};
   int before = 0;
   for (int base = 0; base < l.num_groups; base += 64) {
     const int g = base + lane;
-    const int blocks = g < l.num_groups ? blocks_of(l, groups, g) : 0;
-    const int items = blocks > 0 ? blocks * ((steps_between(0, groups.shared[g]) + per - 1) / per) : 0;
-    const int upto = wave_add_up_to(items);
-    const uint64_t holds = __ballot(before + upto > item);
+    const int blocks = g < l.num_groups ? blocks_of(g) : 0, items = blocks > 0 ? blocks * parts_of(steps_of(plan.shared[g]), per) : 0;
+    const int upto = before + sum_up_to_lane(items);
+    if (g < l.num_groups) plan.before[g] = upto - items;
+    const uint64_t holds = __ballot(upto > wg);
     if (holds != 0) {
       const int at = __ffsll((unsigned long long)holds) - 1;
-      const int place = item - (before + __builtin_amdgcn_readlane(upto - items, at)), row_blocks = __builtin_amdgcn_readlane(blocks, at);
-      return Item{base + at, -1, place % row_blocks, place / row_blocks, per};
+      const int place = wg - __builtin_amdgcn_readlane(upto - items, at), row_blocks = __builtin_amdgcn_readlane(blocks, at), part = quotient(place, row_blocks);
+      found.group = base + at;
+      found.first = __builtin_amdgcn_readfirstlane(plan.start[base + at]);
+      found.count = __builtin_amdgcn_readfirstlane(plan.end[base + at]) - found.first;
+      found.block = place - part * row_blocks;
+      found.from = part * per * STEP;
+      found.to = min(found.from + per * STEP, __builtin_amdgcn_readfirstlane(plan.shared[base + at]));
+      found.at = wg << block_shift;
+      return found;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    before = __builtin_amdgcn_readlane(upto, 63);
   }
+  const int group_items = before;
+  // the sequences' items; every sequence has one at least, which writes down where its rows lie
+  const int item = (wg - group_items) * WAVES + wave;
+  before = 0;
   for (int base = 0; base < l.num_seqs; base += 64) {
     const int b = base + lane;
-    int items = 0;
-    if (b < l.num_seqs) {
-      const Own own = own_of(l, groups, b);
-      items = own_blocks * ((steps_between(own.from, own.to) + per - 1) / per);
-    }
-    const int upto = wave_add_up_to(items);
-    const uint64_t holds = __ballot(before + upto > item);
+    const Own own = base == 0 ? own0 : b < l.num_seqs ? own_of(b) : Own{-1, 0, 0};
+    const int parts = max(1, parts_of(tiles_of(own), per)), items = b < l.num_seqs ? own_blocks * parts : 0;
+    const int upto = before + sum_up_to_lane(items);
+    const uint64_t holds = __ballot(upto > item);
     if (holds != 0) {
       const int at = __ffsll((unsigned long long)holds) - 1;
-      const int place = item - (before + __builtin_amdgcn_readlane(upto - items, at));
-      return Item{-1, base + at, place % own_blocks, place / own_blocks, per};
+      const int first = __builtin_amdgcn_readlane(upto - items, at), place = item - first, part = quotient(place, own_blocks);
+      const int from = __builtin_amdgcn_readlane(own.from, at), to = __builtin_amdgcn_readlane(own.to, at), group = __builtin_amdgcn_readlane(own.group, at);
+      const int low = (from / TILE + part * per) * TILE;
+      found.sequence = base + at;
+      found.block = place - part * own_blocks;
+      found.from = max(low, from);
+      found.to = min(low + per * TILE, to);
+      found.at = (group_items << block_shift) + item * 16;
+      found.tells = place == 0;
+      found.rows.own_at = (group_items << block_shift) + first * 16;
+      found.rows.own_parts = __builtin_amdgcn_readlane(parts, at);
+      if (group >= 0) {
+        found.rows.shared_at = (plan.before[group] << block_shift) + (base + at - plan.start[group]) * l.group;
+        found.rows.shared_stride = blocks_of(group) << block_shift;
+        found.rows.shared_parts = parts_of(steps_of(from), per);
+      }
+      return found;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    before = __builtin_amdgcn_readlane(upto, 63);
   }
-  return Item{-1, -1, 0, 0, per};
+  return found;
 }
 
-// ---- one item ---------------------------------------------------------------------------------------------------------------
+// ---- rows against a stream of keys ----------------------------------------------------------------------------------------
 template <typename T> struct Cache {
   const T* k;
   const T* v;
@@ -194,206 +241,200 @@ template <typename T> struct Cache {
   uint32_t last_page;  // (an id beyond it, which no table should hold, reads this one)
 };
 
-// Row tiles of queries against the keys [lo, hi) of a table's sequence; what they leave goes to part_o[row][D] and part_lse[row].
-// query(row) is the address of a row's query, or nullptr; rows are [first_row, first_row + 16 RT).
-template <typename T, int RT, int DEPTH, typename QueryOf>
-__device__ __forceinline__ void work_item(const Cache<T>& cache, int kvh, const int* __restrict__ table, int lo, int hi, float scale, QueryOf query,
-                                          float* __restrict__ part_o, float* __restrict__ part_lse, char* smem) {
+template <typename T, int RT> struct Rows {  // RT tiles of 16 rows, in a wave
+  static constexpr int NQB = (D + Block<T>::KB - 1) / Block<T>::KB;  // contraction blocks of K Q^T (beyond the head size: zeros)
+  static constexpr int NC = D / 16;
+  float4_t q[RT][NQB], acc[RT][NC];
+  float m[RT], l[RT];  // the running maximum, and this lane's keys' part of the sum
+};
+
+// query(r): the address of row r's query, or nullptr
+template <typename T, int RT, typename QueryOf> __device__ __forceinline__ void begin_rows(Rows<T, RT>& rows, QueryOf query) {
   typedef Block<T> B;
-  constexpr int KB = B::KB, VEC = B::VEC;
-  constexpr int NQB = (D + KB - 1) / KB;   // contraction blocks of K Q^T (beyond the head size: zeros)
-  constexpr int NKB = TILE / KB;           // of V^T P^T
-  constexpr int NC = D / 16;
-  constexpr int IDS = NKB;                 // page ids a lane needs for a tile's keys, and as many for its values
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, i = lane & 15;
-  const int page_size = 1 << cache.page_shift;
-
-  const int tile_lo = lo / TILE, tile_hi = (hi + TILE - 1) / TILE;
-  const int mine = tile_lo + wave;
-
-  // Keys beyond either end are read from the nearest place inside: their scores are masked and their values zeroed.
-  auto key_at = [&](int tile, int u) { return clamped(TILE * tile + B::key_row(u, i), lo, hi - 1); };
-  auto value_at = [&](int tile, int kb) { return clamped(TILE * tile + KB * kb + VEC * g, lo & ~(VEC - 1), (hi - 1) & ~(VEC - 1)); };
-  struct Ids { uint32_t k[IDS], v[IDS]; };
-  auto load_ids = [&](Ids& ids, int tile) {
-#pragma unroll
-    for (int a = 0; a < IDS; ++a) {
-      ids.k[a] = min((uint32_t)table[key_at(tile, a) >> cache.page_shift], cache.last_page);  // (bfloat16: a lane's keys of both score tiles lie in one run of eight)
-      ids.v[a] = min((uint32_t)table[value_at(tile, a) >> cache.page_shift], cache.last_page);
-    }
-  };
-  struct Tile { float4_t k[2][NQB], v[NC][NKB]; };
-  auto load_tile = [&](Tile& x, const Ids& ids, int tile) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int n = key_at(tile, u);
-      const T* p = cache.k + ((((size_t)ids.k[IDS == 1 ? 0 : u] * cache.nkv + kvh) << cache.page_shift) + (n & (page_size - 1))) * D + VEC * g;
-#pragma unroll
-      for (int cb = 0; cb < NQB; ++cb) {
-        // (of a block that reaches beyond the head size, lanes there read the row's beginning and hold zeros)
-        const bool inside = D % KB == 0 || KB * cb + VEC * g < D;
-        x.k[u][cb] = *reinterpret_cast<const float4_t*>(p + (inside ? KB * cb : -VEC * g));
-        if (!inside) x.k[u][cb] = float4_t{0.f, 0.f, 0.f, 0.f};
-      }
-    }
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      const int n = value_at(tile, kb);
-      const T* p = cache.v + ((((size_t)ids.v[kb] * cache.nkv + kvh) * D + i) << cache.page_shift) + (n & (page_size - 1));
-#pragma unroll
-      for (int c = 0; c < NC; ++c) x.v[c][kb] = *reinterpret_cast<const float4_t*>(p + ((size_t)(16 * c) << cache.page_shift));
-    }
-  };
-
-  float4_t qf[RT][NQB], acc[RT][NC];
-  float m_i[RT], l_i[RT];
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const T* q = query(16 * rt + i);
 #pragma unroll
-    for (int cb = 0; cb < NQB; ++cb) {
-      qf[rt][cb] = float4_t{0.f, 0.f, 0.f, 0.f};
-      if (q != nullptr && (D % KB == 0 || KB * cb + VEC * g < D)) qf[rt][cb] = *reinterpret_cast<const float4_t*>(q + KB * cb + VEC * g);
+    for (int cb = 0; cb < Rows<T, RT>::NQB; ++cb) {
+      rows.q[rt][cb] = float4_t{0.f, 0.f, 0.f, 0.f};
+      if (q != nullptr && (D % B::KB == 0 || B::KB * cb + B::VEC * g < D)) rows.q[rt][cb] = *reinterpret_cast<const float4_t*>(q + B::KB * cb + B::VEC * g);
     }
-    m_i[rt] = -INFINITY;
-    l_i[rt] = 0.f;
+    rows.m[rt] = -INFINITY;
+    rows.l[rt] = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc[rt][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < Rows<T, RT>::NC; ++c) rows.acc[rt][c] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
+}
+
+// The rows against those of the keys [lo, hi) of a table's sequence that lie in tiles first, first + stride, ...
+template <typename T, int RT>
+__device__ __forceinline__ void stream_keys(Rows<T, RT>& rows, const Cache<T>& cache, int kvh, const int* __restrict__ table, int lo, int hi, int first, int stride, float scale) {
+  typedef Block<T> B;
+  constexpr int KB = B::KB, VEC = B::VEC, NQB = Rows<T, RT>::NQB, NC = Rows<T, RT>::NC;
+  constexpr int TILE = KB, NU = KB / 16;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int page_size = 1 << cache.page_shift;
+  const int end = (hi + TILE - 1) / TILE;
+  if (first >= end) return;
+  const int last = first + (end - 1 - first) / stride * stride;
+
+  // Keys beyond either end are read from the nearest place inside: their scores are masked and their values zeroed.  (A lane's keys of both
+  // score tiles lie in one run of eight in bfloat16, and so in one page.)
+  auto key_at = [&](int tile, int u) { return clamped(TILE * tile + B::key_row(u, i), lo, hi - 1); };
+  auto value_at = [&](int tile) { return clamped(TILE * tile + VEC * g, lo & ~(VEC - 1), (hi - 1) & ~(VEC - 1)); };
+  struct Ids { uint32_t k[NU], v; };
+  auto load_ids = [&](int tile) {
+    Ids ids;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) ids.k[u] = min((uint32_t)table[key_at(tile, u) >> cache.page_shift], cache.last_page);
+    ids.v = min((uint32_t)table[value_at(tile) >> cache.page_shift], cache.last_page);
+    return ids;
+  };
+  float4_t k[NU][NQB], v[NC];
+  auto load_keys = [&](const Ids& ids, int tile) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int n = key_at(tile, u);
+      const T* p = cache.k + ((((size_t)ids.k[u] * cache.nkv + kvh) << cache.page_shift) + (n & (page_size - 1))) * D + VEC * g;
+#pragma unroll
+      for (int cb = 0; cb < NQB; ++cb) {
+        // (of a block that reaches beyond the head size, lanes there read the row's beginning and hold zeros)
+        const bool inside = D % KB == 0 || KB * cb + VEC * g < D;
+        k[u][cb] = *reinterpret_cast<const float4_t*>(p + (inside ? KB * cb : -VEC * g));
+        if (!inside) k[u][cb] = float4_t{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  };
+  auto load_values = [&](const Ids& ids, int tile) {
+    const int n = value_at(tile);
+    const T* p = cache.v + ((((size_t)ids.v * cache.nkv + kvh) * D + i) << cache.page_shift) + (n & (page_size - 1));
+#pragma unroll
+    for (int c = 0; c < NC; ++c) v[c] = *reinterpret_cast<const float4_t*>(p + ((size_t)(16 * c) << cache.page_shift));
+  };
   const float scale_eff = scale * B::SCALE;
 
-  auto compute = [&](Tile& x, int tile) {
-    const int n0 = TILE * tile;
-    const bool whole = n0 >= lo && n0 + TILE <= hi;  // (the same for the whole wave)
-    if (!whole) {
+  Ids ids = load_ids(first), next_ids = load_ids(min(first + stride, last));
+  load_keys(ids, first);
+  load_values(ids, first);
+  for (int tile = first; tile < end; tile += stride) {
+    const int n0 = TILE * tile, next = min(tile + stride, last);  // (what is asked for behind the last tile is the last tile again)
+    const bool whole = n0 >= lo && n0 + TILE <= hi;               // (the same for the whole wave)
+    float4_t s[RT][NU];
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        const int n = n0 + KB * kb + VEC * g;
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) B::mask(x.v[c][kb], lo - n, hi - n);
+      for (int u = 0; u < NU; ++u) {
+        s[rt][u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int cb = 0; cb < NQB; ++cb) s[rt][u] = B::mma(k[u][cb], rows.q[rt][cb], s[rt][u]);
       }
-    }
-    float4_t pf[RT][NKB];
+    ids = next_ids;
+    next_ids = load_ids(min(tile + 2 * stride, last));
+    load_keys(ids, next);
+    float4_t pf[RT];
     float alpha[RT];
+    bool moved = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float4_t s[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int cb = 0; cb < NQB; ++cb) s[u] = B::mma(x.k[u][cb], qf[rt][cb], s[u]);
-      }
       if (!whole) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int n = n0 + B::first_score(u, g) + j;
-            s[u][j] = n >= lo && n < hi ? s[u][j] : -INFINITY;
+            s[rt][u][j] = n >= lo && n < hi ? s[rt][u][j] : -INFINITY;
           }
       }
       float mx = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[u][j]);
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[rt][u][j]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, VELOX_WAVE));
       mx = fmaxf(mx, __shfl_xor(mx, 32, VELOX_WAVE));
-      const float m_new = fmaxf(m_i[rt], mx * scale_eff);  // (the scale is positive)
+      // What a row's exponents refer to need not be its maximum: it is moved, and all that was gathered rescaled, only when a score lies more than
+      // SLACK above it (bfloat16; in powers of two: weights stay below 2^8, and are rounded relative to themselves).
+      constexpr float SLACK = sizeof(T) == 2 ? 8.f : 0.f;
+      const float top = mx * scale_eff;  // (the scale is positive)
+      const bool stays = top - rows.m[rt] <= SLACK;  // (false while the row has seen no key: -inf)
+      const float m_new = stays ? rows.m[rt] : fmaxf(rows.m[rt], top);
       const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-      alpha[rt] = m_i[rt] == -INFINITY ? 0.f : B::exp_of(m_i[rt] - m_safe);
+      alpha[rt] = stays ? 1.f : rows.m[rt] == -INFINITY ? 0.f : B::exp_of(rows.m[rt] - m_safe);
+      moved = moved || !stays;
       float sum = 0.f;
-      float p[2][4];
+      float p[NU][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          p[u][j] = B::exp_of(fmaf(s[u][j], scale_eff, -m_safe));
+          p[u][j] = B::exp_of(fmaf(s[rt][u][j], scale_eff, -m_safe));
           sum += p[u][j];
         }
       if constexpr (sizeof(T) == 2) {
         bf16x8_t e;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) e[4 * u + j] = (bf16_t)p[u][j];  // probabilities are rounded to the values' type for the product
-        pf[rt][0] = __builtin_bit_cast(float4_t, e);
+          for (int j = 0; j < 4; ++j) e[4 * u + j] = (bf16_t)p[u][j];  // weights are rounded to the values' type for the product
+        pf[rt] = __builtin_bit_cast(float4_t, e);
       } else {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) pf[rt][u < NKB ? u : 0] = float4_t{p[u][0], p[u][1], p[u][2], p[u][3]};
+        pf[rt] = float4_t{p[0][0], p[0][1], p[0][2], p[0][3]};
       }
-      l_i[rt] = l_i[rt] * alpha[rt] + sum;  // of this lane's keys; the four lane groups are added up at the end
-      m_i[rt] = m_new;
+      rows.l[rt] = rows.l[rt] * alpha[rt] + sum;
+      rows.m[rt] = m_new;
     }
-    // the output is rescaled only where a row's maximum moved, which is the exception after a row's first keys
-    bool moved = false;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) moved = moved || alpha[rt] != 1.f;
     if (__ballot(moved) != 0ull) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) acc[rt][c] = acc[rt][c] * alpha[rt];
+        for (int c = 0; c < NC; ++c) rows.acc[rt][c] = rows.acc[rt][c] * alpha[rt];
+    }
+    if (!whole) {
+      const int n = n0 + VEC * g;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) B::mask(v[c], lo - n, hi - n);
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][c] = B::mma(x.v[c][kb], pf[rt][kb], acc[rt][c]);
-  };
-
-  if (mine < tile_hi) {
-    const int last = mine + (tile_hi - 1 - mine) / WAVES * WAVES;  // this wave's last tile
-    Ids ids;
-    load_ids(ids, mine);
-    if constexpr (DEPTH == 2) {
-      // page ids two tiles ahead, keys and values one; what is asked for beyond the last tile is the last tile again
-      Tile ring[2];
-      load_tile(ring[0], ids, mine);
-      load_ids(ids, min(mine + WAVES, last));
-      auto step = [&](int tile, Tile& now, Tile& next) {
-        const int ahead = min(tile + WAVES, last), further = min(tile + 2 * WAVES, last);
-        Ids later;
-        load_ids(later, further);
-        load_tile(next, ids, ahead);
-        ids = later;
-        compute(now, tile);
-      };
-      for (int tile = mine; tile < tile_hi; tile += 2 * WAVES) {
-        step(tile, ring[0], ring[1]);
-        if (tile + WAVES < tile_hi) step(tile + WAVES, ring[1], ring[0]);
-      }
-    } else {
-      Tile x;
-      for (int tile = mine; tile < tile_hi; tile += WAVES) {
-        load_tile(x, ids, tile);
-        load_ids(ids, min(tile + WAVES, last));
-        compute(x, tile);
-      }
-    }
+      for (int rt = 0; rt < RT; ++rt) rows.acc[rt][c] = B::mma(v[c], pf[rt], rows.acc[rt][c]);
+    load_values(ids, next);
   }
+}
 
-  // ---- the four waves' results, a row tile at a time ----
-  float4_t* const acc_all = reinterpret_cast<float4_t*>(smem);                        // [wave][channel tile][lane]
-  float* const m_all = reinterpret_cast<float*>(smem + WAVES * NC * 64 * 16);         // [wave][16 RT]
-  float* const l_all = m_all + WAVES * 16 * RT;
+template <typename T, int RT> __device__ __forceinline__ void finish_sums(Rows<T, RT>& rows) {
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    l_i[rt] += __shfl_xor(l_i[rt], 16, VELOX_WAVE);
-    l_i[rt] += __shfl_xor(l_i[rt], 32, VELOX_WAVE);
+    rows.l[rt] += __shfl_xor(rows.l[rt], 16, VELOX_WAVE);
+    rows.l[rt] += __shfl_xor(rows.l[rt], 32, VELOX_WAVE);
+  }
+}
+
+// The four waves' results of the same rows, put together and written to part_o[row][D] and part_lse[row] (the first `count` rows), a row tile at a time.
+template <int RT> constexpr int join_bytes() { return WAVES * (D / 16) * 64 * 16 + 2 * WAVES * 16 * RT * 4; }
+template <typename T, int RT>
+__device__ __forceinline__ void join_waves(Rows<T, RT>& rows, int count, float* __restrict__ part_o, float* __restrict__ part_lse, char* smem) {
+  typedef Block<T> B;
+  constexpr int NC = D / 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, i = lane & 15;
+  float4_t* const acc_all = reinterpret_cast<float4_t*>(smem);                 // [wave][channel tile][lane]
+  float* const m_all = reinterpret_cast<float*>(smem + WAVES * NC * 64 * 16);  // [wave][16 RT]
+  float* const l_all = m_all + WAVES * 16 * RT;
+  finish_sums<T, RT>(rows);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
     if (g == 0) {
-      m_all[wave * 16 * RT + 16 * rt + i] = m_i[rt];
-      l_all[wave * 16 * RT + 16 * rt + i] = l_i[rt];
+      m_all[wave * 16 * RT + 16 * rt + i] = rows.m[rt];
+      l_all[wave * 16 * RT + 16 * rt + i] = rows.l[rt];
     }
   }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     if (rt > 0) __syncthreads();
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc_all[(wave * NC + c) * 64 + lane] = acc[rt][c];
+    for (int c = 0; c < NC; ++c) acc_all[(wave * NC + c) * 64 + lane] = rows.acc[rt][c];
     __syncthreads();
     float top = -INFINITY, total = 0.f, weight[WAVES];
 #pragma unroll
@@ -410,164 +451,332 @@ __device__ __forceinline__ void work_item(const Cache<T>& cache, int kvh, const 
       float4_t sum = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) sum += acc_all[(w * NC + c) * 64 + lane] * weight[w];
-      *reinterpret_cast<float4_t*>(part_o + (size_t)(16 * rt + i) * D + 16 * c + 4 * g) = sum * inv;
+      if (16 * rt + i < count) *reinterpret_cast<float4_t*>(part_o + (size_t)(16 * rt + i) * D + 16 * c + 4 * g) = sum * inv;
     }
-    if (wave == 0 && g == 0) part_lse[16 * rt + i] = total > 0.f ? top * B::LN_UNIT + logf(total) : -INFINITY;
+    if (wave == 0 && g == 0 && 16 * rt + i < count) part_lse[16 * rt + i] = total > 0.f ? top * B::LN_UNIT + logf(total) : -INFINITY;
   }
 }
 
-template <int RT> constexpr int epilogue_bytes() { return WAVES * (D / 16) * 64 * 16 + 2 * WAVES * 16 * RT * 4; }
+// ---- many rows: tiles in LDS ------------------------------------------------------------------------------------------------------
+// From some hundred rows on the products count, and every 32 rows reading the keys for themselves is more than the second-level caches give.  Here the four
+// waves have 32 rows each and share tiles of 64 keys (bfloat16, heads of 64 and 128 channels).  Every lane asks for 16 bytes of the cache with a
+// load that writes LDS itself, a whole tile ahead of the one being multiplied, into the other of two buffers; one barrier a tile is left.  Such a load fills
+// a contiguous kilobyte, so what lies where is decided by which piece each lane asks for: pieces of 16 bytes change places within a
+// row such that eight lanes that read together touch eight different ones.  Piece c of key k lies at c ^ ((k & 3) | (k >> 3 & 1) << 2), piece c of channel d
+// of V^T, whose rows are the tile's 64 keys, at c ^ (d & 7).
+constexpr int TALL_TILE = 64, TALL_ROWS = 32 * WAVES;
+constexpr bool HAS_TALL = D == 64 || D == 128;
+constexpr int TALL_BYTES = TALL_TILE * D * 2;  // of the keys or the values of a tile
+__device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf16_t>& cache, int kvh, const int* __restrict__ table, int lo, int hi, float scale,
+                                          char (*smem)[2 * TALL_BYTES]) {
+  typedef Block<bf16_t> B;
+  constexpr int CT = 2, NQB = Rows<bf16_t, 2>::NQB, NC = D / 16, NT = TALL_TILE / 16, NKB = TALL_TILE / 32;
+  constexpr int PIECES = D / 8;                  // of a key's row
+  constexpr int LOADS = TALL_BYTES / 1024 / WAVES;  // of a wave, for the keys of a tile, and as many for the values
+  constexpr int KEYS = 64 / PIECES;              // of one load
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, i = lane & 15;
+  const int page_size = 1 << cache.page_shift;
+  // what each lane asks for: of keys KEYS (wave + 4 m) + lane / PIECES, of channels 8 (wave + 4 m) + lane / 8
+  const int key_in_load = lane / PIECES, first_key = KEYS * wave + key_in_load;
+  const uint32_t key_bytes = (uint32_t)(key_in_load * D + 8 * ((lane % PIECES) ^ ((first_key & 3) | ((first_key >> 3) & 1) << 2))) * 2;
+  const int value_eight = (lane & 7) ^ ((lane >> 3) & 7);  // which eight of the tile's keys
+  const size_t page_elems = ((size_t)cache.nkv * D) << cache.page_shift;
+  const uint32_t value_elems = (uint32_t)(kvh * D + 8 * wave + (lane >> 3)) << cache.page_shift;
+  // lane e's page id, e < 8, is that of the tile's keys 8 e .. 8 e + 7, or of the last keys there are
+  auto load_id = [&](int n0) { return min((uint32_t)table[min(n0 + 8 * (lane & 7), hi - 1) >> cache.page_shift], cache.last_page); };
+  auto issue = [&](int n0, uint32_t id, char* to) {
+    const int at = __builtin_amdgcn_readfirstlane(n0);
+#pragma unroll
+    for (int m = 0; m < LOADS; ++m) {
+      const int key0 = KEYS * (wave + WAVES * m);
+      const size_t page = (size_t)(uint32_t)__builtin_amdgcn_readlane(id, key0 >> 3);
+      const bf16_t* base = cache.k + (((page * cache.nkv + kvh) << cache.page_shift) + ((at + key0) & (page_size - 1))) * D;
+      load_to_lds_16(base, key_bytes, to + 1024 * (wave + WAVES * m));
+    }
+    const uint32_t page = __shfl(id, value_eight, VELOX_WAVE);
+    const bf16_t* from = cache.v + (size_t)page * page_elems + (value_elems + (uint32_t)((at + 8 * value_eight) & (page_size - 1)));
+#pragma unroll
+    for (int m = 0; m < LOADS; ++m) load_to_lds_16(from + ((size_t)(8 * WAVES * m) << cache.page_shift), to + TALL_BYTES + 1024 * (wave + WAVES * m));
+  };
+  // where each lane reads its operands: row 8 (i / 4) + i % 4 of a block of 32 keys (+ 4 u for score tile u), pieces 4 cb + g; row i of a channel tile,
+  // pieces 4 kb + g
+  const int half = (i >> 2) & 1;
+  const int key_row = (8 * (i >> 2) + (i & 3)) * (2 * D) + 16 * (g ^ (i & 3)), value_row = TALL_BYTES + i * 128 + 16 * (g ^ (i & 3));
+  const int key_even = key_row + 64 * half, key_odd = key_row + 64 * (1 - half);
+  const int value_first = value_row + 64 * half, value_second = value_row + 64 * (1 - half);
+  const float scale_eff = scale * B::SCALE;
 
-// part_o: [item][KV head][block_rows][D], part_lse: [item][KV head][block_rows]
-template <typename T, int RT, int DEPTH>
-__global__ void __launch_bounds__(64 * WAVES, 1) shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables,
-                                                                      int table_width, const Lengths l, float scale, float* __restrict__ part_o,
-                                                                      float* __restrict__ part_lse) {
-  __shared__ __attribute__((aligned(16))) char smem[sizeof(Groups) > epilogue_bytes<RT>() ? sizeof(Groups) : epilogue_bytes<RT>()];
-  Groups& groups = *reinterpret_cast<Groups*>(smem);
-  load_groups(l, groups);
-  const int kvh = blockIdx.x;
-  const Item item = find_item(l, groups, blockIdx.y);
-  if (item.group < 0 && item.sequence < 0) return;  // (uniform over the workgroup)
-  const size_t slot = ((size_t)blockIdx.y * cache.nkv + kvh) * (16 * RT);
-  float* const o = part_o + slot * D;
-  float* const lse = part_lse + slot;
-  const int group_heads = l.group;
+  // (the queries have arrived before the loop, said in a way the compiler sees: it would otherwise wait for them, and with them for every
+  // load in flight, in every round)
+  uint32_t id = load_id(lo), next_id = load_id(lo + TALL_TILE);
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  issue(lo, id, smem[0]);
+  int buffer = 0;
+  for (int n0 = lo; n0 < hi; n0 += TALL_TILE, buffer ^= 1) {
+    wait_for_loads<0>();  // this wave's pieces of the tile have landed
+    __syncthreads();      // everybody's have, and everybody is done with the other buffer
+    if (n0 + TALL_TILE < hi) {
+      id = next_id;
+      next_id = load_id(n0 + 2 * TALL_TILE);
+      issue(n0 + TALL_TILE, id, smem[buffer ^ 1]);
+    }
+    const char* const tile = smem[buffer];
+    const bool whole = n0 + TALL_TILE <= hi;
+    float4_t s[CT][NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float4_t k[NQB];
+#pragma unroll
+      for (int cb = 0; cb < NQB; ++cb)
+        k[cb] = *reinterpret_cast<const float4_t*>(tile + ((cb & 1) ? key_odd : key_even) + 128 * (cb >> 1) + (32 * (t >> 1) + 4 * (t & 1)) * (2 * D));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int cb = 0; cb < NQB; ++cb)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[ct][t] = B::mma(k[cb], rows.q[ct][cb], s[ct][t]);
+    }
+    float alpha[CT];
+    float4_t pf[CT][NKB];
+    bool moved = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[ct][t][j] = n0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + j < hi ? s[ct][t][j] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[ct][t][j]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, VELOX_WAVE));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, VELOX_WAVE));
+      const float top = mx * scale_eff;
+      const bool stays = top - rows.m[ct] <= 8.f;  // (see stream_keys)
+      const float m_new = stays ? rows.m[ct] : fmaxf(rows.m[ct], top);
+      const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+      alpha[ct] = stays ? 1.f : rows.m[ct] == -INFINITY ? 0.f : B::exp_of(rows.m[ct] - m_safe);
+      moved = moved || !stays;
+      float sum = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        bf16x8_t e;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = B::exp_of(fmaf(s[ct][2 * kb + u][j], scale_eff, -m_safe));
+            sum += p;
+            e[4 * u + j] = (bf16_t)p;
+          }
+        pf[ct][kb] = __builtin_bit_cast(float4_t, e);
+      }
+      rows.l[ct] = rows.l[ct] * alpha[ct] + sum;
+      rows.m[ct] = m_new;
+    }
+    if (__ballot(moved) != 0ull) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = rows.acc[ct][c] * alpha[ct];
+    }
+    float4_t v[2][NKB];  // a channel tile's operands are in flight ahead of the one being multiplied
+    auto read_values = [&](int c, float4_t (&into)[NKB]) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        into[kb] = *reinterpret_cast<const float4_t*>(tile + (kb ? value_second : value_first) + 2048 * c);
+        if (!whole) B::mask(into[kb], 0, hi - (n0 + 32 * kb + 8 * g));
+      }
+    };
+    read_values(0, v[0]);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (c + 1 < NC) read_values(c + 1, v[(c + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = B::mma(v[c & 1][kb], pf[ct][kb], rows.acc[ct][c]);
+    }
+  }
+}
+
+// A wave's rows, put where the joining kernel finds them.
+template <typename T, int RT> __device__ __forceinline__ void leave_rows(Rows<T, RT>& rows, int count, float* __restrict__ part_o, float* __restrict__ part_lse) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  finish_sums<T, RT>(rows);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    if (16 * rt + i >= count) continue;
+    const float inv = rows.l[rt] > 0.f ? 1.f / rows.l[rt] : 1.f;
+    float* const to = part_o + (size_t)(16 * rt + i) * D + 4 * g;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) *reinterpret_cast<float4_t*>(to + 16 * c) = rows.acc[rt][c] * inv;
+    if (g == 0) part_lse[16 * rt + i] = rows.l[rt] > 0.f ? rows.m[rt] * Block<T>::LN_UNIT + logf(rows.l[rt]) : -INFINITY;
+  }
+}
+
+// Two workgroups to a compute unit where a wave's registers allow it.
+template <typename T, int RT> constexpr int workgroups_per_unit() { return D <= 128 && RT * sizeof(T) * D <= 512 ? 2 : 1; }
+
+// part_o: [KV head][rows_room][D], part_lse: [KV head][rows_room]; directory: [sequence]
+// RT = TALL: rows in blocks of TALL_ROWS over tiles in LDS.
+constexpr int TALL = TALL_ROWS / 16;
+template <typename T, int RT>
+__global__ void __launch_bounds__(THREADS, (RT == TALL ? 2 : workgroups_per_unit<T, RT>()))
+shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables, int table_width, const Lengths l, float scale,
+                     float* __restrict__ part_o, float* __restrict__ part_lse, Directory* __restrict__ directory) {
+  constexpr int TILE = Block<T>::KB, R = 16 * RT, ROOM = RT == TALL ? 4 * TALL_BYTES : join_bytes<RT>();
+  __shared__ __attribute__((aligned(1024))) char smem[sizeof(Plan) > ROOM ? sizeof(Plan) : ROOM];
+  const int kvh = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Item item = find_item<TILE>(l, blockIdx.y, *reinterpret_cast<Plan*>(smem));
+  const int heads = l.group;
+  float* const o = part_o + (size_t)kvh * l.rows_room * D;
+  float* const lse = part_lse + (size_t)kvh * l.rows_room;
   if (item.group >= 0) {
-    const int start = groups.start[item.group], rows = (groups.end[item.group] - start) * group_heads, shared = groups.shared[item.group];
-    __syncthreads();  // (the groups' place is used again)
-    const int first_row = item.block * 16 * RT;
-    const int lo = item.part * item.per * STEP, hi = min(lo + item.per * STEP, shared);
-    auto query = [&](int r) -> const T* {
-      const int row = first_row + r;
-      return row < rows ? qkv + (size_t)(start + row / group_heads) * qkv_stride + (size_t)(kvh * group_heads + row % group_heads) * D : nullptr;
+    __syncthreads();  // (the plan's place is used again)
+    if (item.at + R > l.rows_room) return;  // (groups that overlap: no more than there is room for)
+    const int first_row = item.block * R, rows_all = item.count * heads;
+    const int* const table = block_tables + (size_t)item.first * table_width;
+    auto query_of = [&](int row) -> const T* {
+      return row < rows_all ? qkv + (size_t)(item.first + row / heads) * qkv_stride + (size_t)(kvh * heads + row % heads) * D : nullptr;
     };
-    work_item<T, RT, DEPTH>(cache, kvh, block_tables + (size_t)start * table_width, lo, hi, scale, query, o, lse, smem);
-  } else {
-    const Own own = own_of(l, groups, item.sequence);
-    __syncthreads();
-    const int base = own.from / TILE * TILE + item.part * item.per * STEP;
-    const int lo = max(base, own.from), hi = min(base + item.per * STEP, own.to);
-    auto query = [&](int r) -> const T* {
-      const int row = item.block * 16 + r;
-      return row < group_heads ? qkv + (size_t)item.sequence * qkv_stride + (size_t)(kvh * group_heads + row) * D : nullptr;
-    };
-    work_item<T, 1, 2 * sizeof(T) * D <= 1024 ? 2 : 1>(cache, kvh, block_tables + (size_t)item.sequence * table_width, lo, hi, scale, query, o, lse, smem);
-  }
-}
-
-// A workgroup per (sequence, KV head): the items that hold its rows, joined.  A sink adds exp(sink) to the denominator.
-constexpr int MERGE_THREADS = 256;
-template <typename T>
-__global__ void __launch_bounds__(MERGE_THREADS) shared_prefix_merge_kernel(const Lengths l, int nkv, const float* __restrict__ part_o, const float* __restrict__ part_lse,
-                                                                            const float* __restrict__ sinks, T* __restrict__ out, int items_room) {
-  __shared__ Groups groups;
-  load_groups(l, groups);
-  const int kvh = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, own_blocks = (l.group + 15) / 16;
-  const int per = steps_per_item(l, groups);
-  const Own own = own_of(l, groups, b);
-  // items before this sequence's group, of all groups, and of the sequences before this one
-  int before_group = 0, before_own = 0;
-  for (int g = lane; g < l.num_groups; g += 64) {
-    const int items = blocks_of(l, groups, g) * ((steps_between(0, groups.shared[g]) + per - 1) / per);
-    before_own += items;
-    before_group += g < own.group ? items : 0;
-  }
-  for (int s = lane; s < b; s += 64) {
-    const Own other = own_of(l, groups, s);
-    before_own += own_blocks * ((steps_between(other.from, other.to) + per - 1) / per);
-  }
-  before_group = wave_add(before_group);
-  before_own = wave_add(before_own);
-  const int shared_blocks = own.group >= 0 ? blocks_of(l, groups, own.group) : 0;
-  const int shared_parts = own.group >= 0 ? (steps_between(0, own.from) + per - 1) / per : 0;
-  const int own_parts = (steps_between(own.from, own.to) + per - 1) / per;
-  const int first_row = own.group >= 0 ? (b - groups.start[own.group]) * l.group : 0;
-  constexpr int QUADS = D / 4;
-  for (int at = threadIdx.x; at < l.group * QUADS; at += MERGE_THREADS) {
-    const int h = at / QUADS, channel = at % QUADS * 4;
-    const int row = first_row + h;
-    auto place_of = [&](int part) -> size_t {  // of this head's row in the part's item
-      const int item = part < shared_parts ? before_group + part * shared_blocks + row / l.block_rows : before_own + (part - shared_parts) * own_blocks + h / 16;
-      const int r = part < shared_parts ? row % l.block_rows : h % 16;
-      return ((size_t)min(item, items_room - 1) * nkv + kvh) * l.block_rows + r;
-    };
-    float top = -INFINITY, denom = 0.f;
-    float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
-    constexpr int ROUND = 8;
-    const int parts = shared_parts + own_parts;
-    for (int p0 = 0; p0 < parts; p0 += ROUND) {
-      float logs[ROUND];
-      float4_t o[ROUND];
-#pragma unroll
-      for (int j = 0; j < ROUND; ++j) {
-        const size_t place = place_of(min(p0 + j, parts - 1));
-        logs[j] = p0 + j < parts ? part_lse[place] : -INFINITY;
-        o[j] = *reinterpret_cast<const float4_t*>(part_o + place * D + channel);
-      }
-      float now = top;
-#pragma unroll
-      for (int j = 0; j < ROUND; ++j) now = fmaxf(now, logs[j]);
-      const float safe = now == -INFINITY ? 0.f : now, old = top == -INFINITY ? 0.f : expf(top - safe);
-      denom *= old;
-      acc = acc * old;
-      top = now;
-#pragma unroll
-      for (int j = 0; j < ROUND; ++j) {
-        if (logs[j] == -INFINITY) continue;  // (what was asked for again may be anything)
-        const float weight = expf(logs[j] - safe);
-        denom += weight;
-        acc += o[j] * weight;
-      }
+    if constexpr (RT == TALL) {
+      const int wave_row = 32 * wave;
+      Rows<T, 2> rows;
+      begin_rows<T, 2>(rows, [&](int r) { return query_of(first_row + wave_row + r); });
+      tall_item(rows, cache, kvh, table, item.from, item.to, scale, reinterpret_cast<char(*)[2 * TALL_BYTES]>(smem));
+      leave_rows<T, 2>(rows, rows_all - first_row - wave_row, o + (size_t)(item.at + wave_row) * D, lse + item.at + wave_row);
+      return;
+    } else {
+    Rows<T, RT> rows;
+    begin_rows<T, RT>(rows, [&](int r) { return query_of(first_row + r); });
+    stream_keys<T, RT>(rows, cache, kvh, table, item.from, item.to, item.from / TILE + wave, WAVES, scale);
+    join_waves<T, RT>(rows, rows_all - first_row, o + (size_t)item.at * D, lse + item.at, smem);
+    return;
     }
-    const int head = kvh * l.group + h;
-    if (sinks != nullptr && top != -INFINITY) denom += expf(sinks[head] - top);
-    const float4_t result = acc * (denom > 0.f ? 1.f / denom : 1.f);
-    T* dst = out + ((size_t)b * l.group * nkv + head) * D + channel;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) dst[j] = from_f32<T>(result[j]);
   }
+  if (item.sequence < 0 || item.at + 16 > l.rows_room) return;
+  if (item.tells && kvh == 0 && lane == 0) directory[item.sequence] = item.rows;
+  Rows<T, 1> rows;
+  begin_rows<T, 1>(rows, [&](int r) -> const T* {
+    const int row = item.block * 16 + r;
+    return row < heads ? qkv + (size_t)item.sequence * qkv_stride + (size_t)(kvh * heads + row) * D : nullptr;
+  });
+  if (item.to > item.from)
+    stream_keys<T, 1>(rows, cache, kvh, block_tables + (size_t)item.sequence * table_width, item.from, item.to, item.from / TILE, 1, scale);
+  leave_rows<T, 1>(rows, heads - 16 * item.block, o + (size_t)item.at * D, lse + item.at);
 }
 
-// Row tiles a wave can hold: its registers hold the queries, the output and two tiles of keys and values.
-template <typename T> constexpr int most_row_tiles() { return sizeof(T) * D <= 256 ? 4 : sizeof(T) * D <= 512 ? 2 : 1; }
+// A wave per (head, sequence): the parts that hold its row, joined.  Lane p asks for part p's log-sum (the next 64 parts', if there are more, in
+// another round) and every lane for its own channels of up to AHEAD parts, all before it waits for any of them.  A sink adds exp(sink) to the
+// denominator.
+constexpr int LANE_CHANNELS = D <= 64 ? 1 : D <= 128 ? 2 : 4, JOIN_HEADS = 4;
+template <typename T>
+__global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int nh, int group, int rows_room, const Directory* __restrict__ directory,
+                                                                             const float* __restrict__ part_o, const float* __restrict__ part_lse,
+                                                                             const float* __restrict__ sinks, T* __restrict__ out) {
+  typedef float channels_t __attribute__((ext_vector_type(LANE_CHANNELS)));
+  constexpr int AHEAD = 64 / LANE_CHANNELS < 32 ? 64 / LANE_CHANNELS : 32;
+  const int lane = threadIdx.x & 63, head = blockIdx.x * JOIN_HEADS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.y;
+  if (head >= nh) return;
+  const Directory d = directory[b];
+  const int kvh = head / group, h = head - kvh * group, own_stride = (group + 15) / 16 * 16;
+  const int shared_parts = clamped(d.shared_parts, 0, rows_room / 16), parts = shared_parts + clamped(d.own_parts, 0, rows_room / 16);  // (of groups that overlap nobody
+  auto place_of = [&](int part) -> size_t {                                                                                             // may have written it down)
+    const unsigned row = part < shared_parts ? (unsigned)d.shared_at + (unsigned)part * (unsigned)d.shared_stride
+                                             : (unsigned)d.own_at + (unsigned)(part - shared_parts) * (unsigned)own_stride;
+    return (size_t)kvh * rows_room + min(row + (unsigned)h, (unsigned)rows_room - 1u);
+  };
+  const bool live = lane * LANE_CHANNELS < D;
+  const float* const channels = part_o + (live ? lane * LANE_CHANNELS : 0);
+  float top = -INFINITY, denom = 0.f;
+  channels_t acc = 0.f;
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    const int here = min(parts - p0, 64);
+    const float log_sum = lane < here ? part_lse[place_of(p0 + lane)] : -INFINITY;
+    channels_t o[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      o[j] = *reinterpret_cast<const channels_t*>(channels + place_of(p0 + (j < here ? j : here - 1)) * D);  // (no branch, or each would wait for the one before)
+    const float now = fmaxf(top, wave_max(log_sum)), safe = now == -INFINITY ? 0.f : now, old = top == -INFINITY ? 0.f : expf(top - safe);
+    const float weight = log_sum == -INFINITY ? 0.f : expf(log_sum - safe);
+    denom = denom * old + wave_sum(weight);
+    acc = acc * old;
+    top = now;
+    auto weight_of = [&](int j) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), j)); };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      acc += (j < here ? o[j] : channels_t(0.f)) * weight_of(j);  // (a part without a key holds zeros)
+    for (int j = AHEAD; j < here; ++j) acc += *reinterpret_cast<const channels_t*>(channels + place_of(p0 + j) * D) * weight_of(j);
+  }
+  if (sinks != nullptr && top != -INFINITY) denom += expf(sinks[head] - top);
+  if (!live) return;
+  acc = acc * (denom > 0.f ? 1.f / denom : 1.f);
+  T* const dst = out + ((size_t)b * nh + head) * D + lane * LANE_CHANNELS;
+#pragma unroll
+  for (int j = 0; j < LANE_CHANNELS; ++j) dst[j] = from_f32<T>(acc[j]);
+}
+
+// Row tiles a wave can hold: its registers hold the queries, the output and a tile of keys and values.
+template <typename T> constexpr int most_row_tiles() { return sizeof(T) * D <= 128 ? 4 : D <= 128 ? 2 : 1; }
 
 extern "C" int velox_shared_prefix_head_dim() { return D; }
+extern "C" int velox_shared_prefix_tall(int dtype) { return dtype == VELOX_BF16 && HAS_TALL ? TALL : 0; }
 extern "C" int velox_shared_prefix_most_row_tiles(int dtype) { return dtype == VELOX_BF16 ? most_row_tiles<bf16_t>() : most_row_tiles<float>(); }
 
 template <typename T>
 static int launch(const void* qkv, int qkv_stride, const void* k_cache, const void* v_cache, const int* block_tables, int table_width, const Lengths& l, int row_tiles,
-                  int items, const float* sinks, void* out, float* part_o, float* part_lse, int nkv, int page_shift, int pages, float scale, hipStream_t stream) {
+                  int items, const float* sinks, void* out, float* part_o, float* part_lse, Directory* directory, int nkv, int page_shift, int pages, float scale,
+                  hipStream_t stream) {
   const Cache<T> cache{(const T*)k_cache, (const T*)v_cache, nkv, page_shift, (uint32_t)(pages - 1)};
-  constexpr int DEPTH = sizeof(T) * D <= 512 ? 2 : 1, MOST = most_row_tiles<T>();
-  const dim3 grid(nkv, items);
-  if (row_tiles == 1) shared_prefix_kernel<T, 1, DEPTH><<<grid, 64 * WAVES, 0, stream>>>((const T*)qkv, qkv_stride, cache, block_tables, table_width, l, scale, part_o, part_lse);
+  constexpr int MOST = most_row_tiles<T>();
+  auto kernel = shared_prefix_kernel<T, 1>;
   if constexpr (MOST >= 2) {
-    if (row_tiles == 2) shared_prefix_kernel<T, 2, DEPTH><<<grid, 64 * WAVES, 0, stream>>>((const T*)qkv, qkv_stride, cache, block_tables, table_width, l, scale, part_o, part_lse);
+    if (row_tiles == 2) kernel = shared_prefix_kernel<T, 2>;
   }
   if constexpr (MOST >= 4) {
-    if (row_tiles == 4) shared_prefix_kernel<T, 4, DEPTH><<<grid, 64 * WAVES, 0, stream>>>((const T*)qkv, qkv_stride, cache, block_tables, table_width, l, scale, part_o, part_lse);
+    if (row_tiles == 4) kernel = shared_prefix_kernel<T, 4>;
   }
+  if constexpr (HAS_TALL && sizeof(T) == 2) {
+    if (row_tiles == TALL) kernel = shared_prefix_kernel<T, TALL>;
+  }
+  kernel<<<dim3(nkv, items), THREADS, 0, stream>>>((const T*)qkv, qkv_stride, cache, block_tables, table_width, l, scale, part_o, part_lse, directory);
   const int status = (int)hipGetLastError();
   if (status != 0) return status;
-  shared_prefix_merge_kernel<T><<<dim3(nkv, l.num_seqs), MERGE_THREADS, 0, stream>>>(l, nkv, part_o, part_lse, sinks, (T*)out, items);
+  shared_prefix_join_kernel<T><<<dim3((nkv * l.group + JOIN_HEADS - 1) / JOIN_HEADS, l.num_seqs), 64 * JOIN_HEADS, 0, stream>>>(nkv * l.group, l.group, l.rows_room, directory, part_o, part_lse, sinks, (T*)out);
   return (int)hipGetLastError();
 }
 
-// items: at least the most there can be, one more for every row block than its share of `target`: at most num_seqs G / (16 row_tiles) +
-// num_groups of the groups' and num_seqs ceil(G / 16) of the sequences'.  most_keys: no length counts beyond it.  part_o: float32 [items, nkv, 16 row_tiles, D], part_lse the same without D.
+// items: workgroups per KV head, and rows_room: rows per KV head, at least what velox_shared_prefix_room gives.  part_o: float32 [nkv, rows_room, D],
+// part_lse: float32 [nkv, rows_room], directory: eight int32 a sequence.  most_keys: no length counts beyond it.
+// An item has as many steps as the whole over `target`, the last of every row block fewer: at most `target` items and one for every row block, of which
+// the groups have num_seqs G / block_rows + num_groups at most and the sequences num_seqs ceil(G / 16), a quarter of a workgroup each.
+extern "C" void velox_shared_prefix_room(int num_seqs, int num_groups, int group, int row_tiles, int target, long long* items, long long* rows) {
+  const long long block_rows = 16LL * row_tiles, own_blocks = (long long)num_seqs * ((group + 15) / 16), blocks = (long long)num_seqs * group / block_rows + num_groups;
+  *items = target + blocks + own_blocks / WAVES + 2;
+  *rows = target * (block_rows > 16 * WAVES ? block_rows : 16 * WAVES) + blocks * block_rows + own_blocks * 16 + 16 * WAVES;
+}
 extern "C" int velox_shared_prefix_attention(const void* qkv, int qkv_stride, const void* k_cache, const void* v_cache, const int* block_tables, int table_width,
                                              const int* kv_lens, const int* group_starts, const int* shared_lens, int num_seqs, int num_groups, int nh, int nkv,
-                                             int page_shift, int pages, int most_keys, float scale, int row_tiles, int target, int items, const float* sinks, void* out, float* part_o, float* part_lse,
-                                             int dtype, hipStream_t stream) {
+                                             int page_shift, int pages, int most_keys, float scale, int row_tiles, int target, long long items, long long rows_room,
+                                             const float* sinks, void* out, float* part_o, float* part_lse, int* directory, int dtype, hipStream_t stream) {
   if (num_seqs <= 0) return 0;
-  if (nkv < 1 || nh % nkv != 0 || page_shift < 3 || pages < 1 || most_keys < 0 || most_keys > (long long)table_width << page_shift || num_groups < 0 || num_groups > MOST_GROUPS || target < 1 || num_seqs > 65535 || items > 65535) return -1;
-  if (row_tiles < 1 || row_tiles == 3 || row_tiles > velox_shared_prefix_most_row_tiles(dtype)) return -1;
+  if (nkv < 1 || nh % nkv != 0 || page_shift < 3 || pages < 1 || most_keys < 0 || most_keys > (long long)table_width << page_shift || num_groups < 0 ||
+      num_groups > MOST_GROUPS || target < 1 || num_seqs > 65535 || items > 65535 || rows_room > 0x7fffffffLL) return -1;
+  if (row_tiles < 1 || (row_tiles & (row_tiles - 1)) != 0 || (row_tiles > velox_shared_prefix_most_row_tiles(dtype) && row_tiles != velox_shared_prefix_tall(dtype))) return -1;
   const int group = nh / nkv;
-  const long long most = (long long)target + (long long)num_seqs * group / (16 * row_tiles) + num_groups + (long long)num_seqs * ((group + 15) / 16);
-  if (items < most) return -1;
-  const Lengths l{kv_lens, group_starts, shared_lens, num_seqs, num_groups, group, 16 * row_tiles, target, most_keys};
+  long long least_items, least_rows;
+  velox_shared_prefix_room(num_seqs, num_groups, group, row_tiles, target, &least_items, &least_rows);
+  if (items < least_items || rows_room < least_rows) return -1;
+  const Lengths l{kv_lens, group_starts, shared_lens, num_seqs, num_groups, group, 16 * row_tiles, target, most_keys, (int)rows_room};
   if (dtype == VELOX_BF16)
-    return launch<bf16_t>(qkv, qkv_stride, k_cache, v_cache, block_tables, table_width, l, row_tiles, items, sinks, out, part_o, part_lse, nkv, page_shift, pages, scale, stream);
-  return launch<float>(qkv, qkv_stride, k_cache, v_cache, block_tables, table_width, l, row_tiles, items, sinks, out, part_o, part_lse, nkv, page_shift, pages, scale, stream);
+    return launch<bf16_t>(qkv, qkv_stride, k_cache, v_cache, block_tables, table_width, l, row_tiles, (int)items, sinks, out, part_o, part_lse, (Directory*)directory, nkv,
+                          page_shift, pages, scale, stream);
+  return launch<float>(qkv, qkv_stride, k_cache, v_cache, block_tables, table_width, l, row_tiles, (int)items, sinks, out, part_o, part_lse, (Directory*)directory, nkv,
+                       page_shift, pages, scale, stream);
 }

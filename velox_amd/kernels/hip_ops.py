@@ -276,7 +276,8 @@ class HipOps:
         lib = self._shared_prefix.get(head_dim)
         if lib is None:
             lib = ctypes.CDLL(build.ensure_shared_prefix(head_dim))
-            lib.velox_shared_prefix_attention.argtypes = [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P, _P, _I, _P]
+            lib.velox_shared_prefix_attention.argtypes = [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, ctypes.c_longlong, ctypes.c_longlong, _P, _P,
+                                                          _P, _P, _P, _I, _P]
             lib.velox_shared_prefix_most_row_tiles.argtypes = [_I]
             for fn in (lib.velox_shared_prefix_attention, lib.velox_shared_prefix_most_row_tiles, lib.velox_shared_prefix_head_dim):
                 fn.restype = _I
@@ -2300,15 +2301,19 @@ class HipOps:
     MAX_BEAMS, MAX_KEPT, MAX_BEAM_VOCAB = 256, 64, 1 << 24  # of ``beam_select``
     MAX_MOVED = 64  # beams of a request that ``reorder_states`` moves
 
-    def _shared_prefix_shape(self, num_seqs: int, num_groups: int, num_heads: int, num_kv_heads: int, head_dim: int, element_size: int, largest_group: int) -> Tuple[int, int, int]:
-        """Row tiles of a workgroup, over how many workgroups per KV head the keys are cut, and the most items that makes."""
+    def _shared_prefix_shape(self, num_seqs: int, num_groups: int, num_heads: int, num_kv_heads: int, head_dim: int, element_size: int, largest_group: int) -> Tuple[int, int, int, int]:
+        """Row tiles of a workgroup, over how many workgroups per KV head the keys are cut, and how many workgroups and rows of partial results
+        per KV head that makes at most (as ``velox_shared_prefix_room`` counts them)."""
         group = num_heads // num_kv_heads
-        most = 4 if element_size * head_dim <= 256 else 2 if element_size * head_dim <= 512 else 1
+        most = 4 if element_size * head_dim <= 128 else 2 if head_dim <= 128 else 1
         row_tiles = 1
         while row_tiles < most and 16 * row_tiles < largest_group * group:
             row_tiles *= 2
-        target = max(1, self.num_cus // num_kv_heads)
-        return row_tiles, target, target + num_seqs * group // (16 * row_tiles) + num_groups + num_seqs * (-(-group // 16))
+        if element_size == 2 and head_dim in (64, 128) and largest_group * group > 64:
+            row_tiles = 8
+        target = max(1, 2 * self.num_cus // num_kv_heads)
+        own_blocks, blocks = num_seqs * (-(-group // 16)), num_seqs * group // (16 * row_tiles) + num_groups
+        return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(16 * row_tiles, 64) + blocks * 16 * row_tiles + own_blocks * 16 + 64
 
     def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> Tuple[int, int]:
         """The most float32 elements ``shared_prefix_attention`` asks its workspace for (``shared_prefix_out``, ``shared_prefix_lse``) in any
@@ -2316,9 +2321,9 @@ class HipOps:
         rows = 0
         for element_size in (2, 4):
             for largest in (1, 1 << 20):
-                row_tiles, _, items = self._shared_prefix_shape(max_num_seqs, max_num_groups, num_heads, num_kv_heads, head_dim, element_size, largest)
-                rows = max(rows, items * num_kv_heads * 16 * row_tiles)
-        return rows * head_dim, rows
+                for groups in (0, max_num_groups):
+                    rows = max(rows, self._shared_prefix_shape(max_num_seqs, groups, num_heads, num_kv_heads, head_dim, element_size, largest)[3])
+        return rows * num_kv_heads * head_dim, rows * num_kv_heads + 8 * max_num_seqs
 
     def shared_prefix_attention(self, qkv, num_heads, num_kv_heads, head_dim, k_cache, v_cache, block_size, block_tables, kv_lens, group_starts, shared_lens,
                                 largest_group, max_kv_len, scale, workspace, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2372,18 +2377,17 @@ class HipOps:
         out = torch.empty((num_seqs, num_heads * head_dim), dtype=qkv.dtype, device=self.device)
         if num_seqs == 0:
             return out
-        row_tiles, target, items = self._shared_prefix_shape(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, qkv.element_size(), int(largest_group))
+        row_tiles, target, items, rows = self._shared_prefix_shape(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, qkv.element_size(), int(largest_group))
         if items > 65535 or num_seqs > 65535:
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
-        rows = items * num_kv_heads * 16 * row_tiles
-        part_o = workspace.get("shared_prefix_out", rows * head_dim)
-        part_lse = workspace.get("shared_prefix_lse", rows)
+        part_o = workspace.get("shared_prefix_out", rows * num_kv_heads * head_dim)
+        part_lse = workspace.get("shared_prefix_lse", rows * num_kv_heads + 8 * num_seqs)  # (and where the sequences' rows lie, eight numbers each)
         lib = self.shared_prefix_library(head_dim)
         with self._current():
             status = lib.velox_shared_prefix_attention(
                 _ptr(qkv), width, _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(kv_lens), _ptr(group_starts), _ptr(shared_lens), num_seqs,
-                num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages, int(max_kv_len), float(scale), row_tiles, target, items, _ptr(sinks), _ptr(out), _ptr(part_o), _ptr(part_lse),
-                dtype, self._stream())
+                num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages, int(max_kv_len), float(scale), row_tiles, target, items, rows, _ptr(sinks), _ptr(out),
+                _ptr(part_o), _ptr(part_lse), _ptr(part_lse[rows * num_kv_heads:]), dtype, self._stream())
         self._launched(status, "shared_prefix_attention")
         return out
 
