@@ -17,6 +17,7 @@ def ops():
     """The checks alone: no library, so that anything that passes them says so."""
     made = object.__new__(HipOps)
     made.device = torch.device("cpu")
+    made._index = -1
     made.num_cus = 256
     made._raw_stream = None
     made._shared_prefix = {dim: _Nothing() for dim in range(16, 272, 16)}
@@ -57,8 +58,8 @@ def attention(**changed):
     (dict(max_kv_len=-1), "cannot cover"),
     (dict(kv_lens=torch.ones(3, dtype=torch.int64)), "kv_lens"),
     (dict(kv_lens=torch.ones((3, 1), dtype=torch.int32)), "kv_lens"),
-    (dict(group_starts=torch.tensor([0, 1, 3], dtype=torch.int32)), "starts"),
-    (dict(shared_lens=torch.tensor([[1]], dtype=torch.int32)), "starts"),
+    (dict(group_starts=torch.tensor([0, 1, 3], dtype=torch.int32)), "group_starts"),
+    (dict(shared_lens=torch.tensor([[1]], dtype=torch.int32)), "shared_lens"),
     (dict(group_starts=torch.zeros(1026, dtype=torch.int32), shared_lens=torch.zeros(1025, dtype=torch.int32)), "at most 1024"),
     (dict(largest_group=0), "largest group"),
     (dict(largest_group=4), "largest group"),
@@ -91,7 +92,7 @@ def test_attention_items_are_enough(ops, heads, kv_heads, dim):
         num_seqs = max(1, sum(sizes) + rng.randint(0, 5))
         element_size = rng.choice([2, 4])
         tile = 32 if element_size == 2 else 16
-        row_tiles, target, items, rows = ops._shared_prefix_shape(num_seqs, len(sizes), heads, kv_heads, dim, element_size, max(sizes + [1]))
+        row_tiles, target, items, rows = ops._shared_prefix_shape(256, num_seqs, len(sizes), heads, kv_heads, dim, element_size, max(sizes + [1]))
         own_blocks = -(-group // 16)
         shared_work, own_work = [], []  # (row blocks, steps) of the groups, tiles of the sequences
         for size in sizes:

@@ -254,9 +254,7 @@ def test_attention_scratch_is_what_it_says(ops):
     """A workspace of the stated size, fixed, serves every step within its limits."""
     for heads, kv_heads, dim, page in SHAPES:
         workspace = Workspace(torch.device("cuda"))
-        out, lse = ops.shared_prefix_scratch_elems(heads, kv_heads, dim, 40, 6)
-        workspace.reserve("shared_prefix_out", out)
-        workspace.reserve("shared_prefix_lse", lse)
+        workspace.reserve("shared_prefix_parts", ops.shared_prefix_scratch_elems(heads, kv_heads, dim, 40, 6))
         workspace.fix()
         for dtype in (BF16, F32):
             for groups, lens, behind in ([(40, 33)], own(40, 33, 1, 3), 0), ([(2, 100)] * 6, own(12, 100, 1, 3), 0), ([], [5], 1):

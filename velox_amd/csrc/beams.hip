@@ -533,43 +533,48 @@ struct MovedTensor {
 };
 struct MovedTensors { MovedTensor of[MOST_TENSORS]; };
 
-// Grid (columns, request and place, outer runs of all tensors); a column is WIDTH bytes.
+// Grid (columns, request and place, outer runs of all tensors); a column is as many bytes as a Column.  Every row that anybody takes over is
+// read once, whoever takes it.
 template <typename Column, int MOST>
-__global__ void __launch_bounds__(THREADS) reorder_kernel(const MovedTensors tensors, int count, const int* __restrict__ slots, const int* __restrict__ parents, int beams,
-                                                          int places) {
+__global__ void __launch_bounds__(THREADS, MOST <= 8 ? 8 : MOST <= 16 ? 4 : MOST <= 32 ? 2 : 1)
+reorder_kernel(const MovedTensors tensors, int count, const int* __restrict__ slots, const int* __restrict__ parents, int beams, int places) {
   int at = 0;
   for (int t = 1; t < count; ++t) at = (int)blockIdx.z >= tensors.of[t].outer_before ? t : at;
   const MovedTensor tensor = tensors.of[at];
-  const long long column = ((long long)blockIdx.x * THREADS + threadIdx.x) * (long long)sizeof(Column);
   if ((long long)blockIdx.x * THREADS * (long long)sizeof(Column) >= tensor.row_bytes) return;
+  const long long column = ((long long)blockIdx.x * THREADS + threadIdx.x) * (long long)sizeof(Column);
   const int request = blockIdx.y / places, place = blockIdx.y % places, lane = threadIdx.x & 63;
-  // lane j: where beam j's row lies and where its parent's does
-  int row = -1, from = -1;
+  // lane j: beam j's parent, its row, and whether it takes over another one
+  int parent = -1, row = -1;
   if (lane < beams) {
+    parent = parents[(long long)request * beams + lane];
     row = slots[((long long)request * beams + lane) * places + place];
-    const int parent = parents[(long long)request * beams + lane];
-    from = parent >= 0 && parent < beams ? slots[((long long)request * beams + parent) * places + place] : -1;
   }
-  uint64_t moving = __ballot(row >= 0 && row < tensor.rows && from >= 0 && from < tensor.rows && from != row);
-  if (column >= tensor.row_bytes) return;
+  const bool there = row >= 0 && row < tensor.rows;
+  const uint64_t rows_there = __ballot(there);
+  const bool moves = there && parent >= 0 && parent < beams && (rows_there >> (parent & 63) & 1) != 0 && __shfl(row, parent & 63, VELOX_WAVE) != row;
+  uint64_t taken = 0;
+  for (uint64_t left = __ballot(moves); left != 0; left &= left - 1) taken |= 1ull << __builtin_amdgcn_readlane(parent, __ffsll((unsigned long long)left) - 1);
+  if (taken == 0) return;
+  const bool live = column < tensor.row_bytes;
   char* const base = tensor.base + (long long)((int)blockIdx.z - tensor.outer_before) * tensor.outer_bytes + column;
+  auto row_at = [&](int beam) { return base + (long long)__builtin_amdgcn_readlane(row, beam) * tensor.row_bytes; };
   Column held[MOST];
-  uint64_t todo = moving;
+  uint64_t todo = taken;
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
     if (todo != 0) {
-      const int j = __ffsll((unsigned long long)todo) - 1;
+      if (live) held[k] = __builtin_nontemporal_load(reinterpret_cast<const Column*>(row_at(__ffsll((unsigned long long)todo) - 1)));
       todo &= todo - 1;
-      held[k] = *reinterpret_cast<const Column*>(base + (long long)__builtin_amdgcn_readlane(from, j) * tensor.row_bytes);
     }
   }
-  todo = moving;
+  todo = taken;
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
     if (todo != 0) {
-      const int j = __ffsll((unsigned long long)todo) - 1;
+      for (uint64_t to = __ballot(moves && parent == __ffsll((unsigned long long)todo) - 1); to != 0; to &= to - 1)
+        if (live) __builtin_nontemporal_store(held[k], reinterpret_cast<Column*>(row_at(__ffsll((unsigned long long)to) - 1)));
       todo &= todo - 1;
-      *reinterpret_cast<Column*>(base + (long long)__builtin_amdgcn_readlane(row, j) * tensor.row_bytes) = held[k];
     }
   }
 }

@@ -20,6 +20,8 @@
 // indices (32 in bfloat16, 16 in float32) lane (g = lane / 16, i = lane % 16) holds 16 bytes of row or column i, those of place g; a result is rows
 // 4 g .. 4 g + 3 of column i.  In bfloat16 row 4 q + j of the tile's score tile u (q, j < 4) is key 8 q + 4 u + j, so that a lane's
 // scores of both are those of keys 8 g .. 8 g + 7: the operand of the second product, and one load of V^T.
+#include <type_traits>
+
 #include "common.h"
 
 #ifndef VELOX_HEAD_DIM
@@ -92,6 +94,7 @@ struct Plan {  // in LDS
   int start[MOST_GROUPS], end[MOST_GROUPS], shared[MOST_GROUPS];
   int before[MOST_GROUPS];  // items of the groups before
   int lens[LENS_HELD];
+  int begins[LENS_HELD];    // 1 + the group that begins at a sequence, or 0
 };
 struct Directory { int shared_at, shared_stride, shared_parts, own_at, own_parts, unused[3]; };  // of a sequence: where its rows lie
 struct Item {           // group >= 0: of that group's shared keys, by the whole workgroup; else sequence >= 0: of its own keys, by this wave; else none
@@ -104,6 +107,18 @@ struct Item {           // group >= 0: of that group's shared keys, by the whole
 };
 
 __device__ __forceinline__ int clamped(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+// the greatest of v >= 0 and those of the lanes before
+__device__ __forceinline__ int most_up_to_lane(int v) {
+#define VELOX_MAX_SHIFTED(CONTROL, ROWS) v = max(v, __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false))
+  VELOX_MAX_SHIFTED(0x111, 0xf);
+  VELOX_MAX_SHIFTED(0x112, 0xf);
+  VELOX_MAX_SHIFTED(0x114, 0xf);
+  VELOX_MAX_SHIFTED(0x118, 0xf);
+  VELOX_MAX_SHIFTED(0x142, 0xa);
+  VELOX_MAX_SHIFTED(0x143, 0xc);
+#undef VELOX_MAX_SHIFTED
+  return v;
+}
 // a / b rounded down, 0 <= a < 2^23 <= 2^31 / b: by the reciprocal, which is off by one at most
 __device__ __forceinline__ int quotient(int a, int b) {
   int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
@@ -144,34 +159,49 @@ __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) 
     shared0 = l.shared_lens[g];
   }
   const int len0 = l.kv_lens[at_most(lane, l.num_seqs)];
-  for (int b = lane; b < l.num_seqs && b < LENS_HELD; b += 64) plan.lens[b] = clamped(b < 64 ? len0 : l.kv_lens[b], 0, l.most);
+  for (int b = lane; b < l.num_seqs && b < LENS_HELD; b += 64) {
+    plan.lens[b] = clamped(b < 64 ? len0 : l.kv_lens[b], 0, l.most);
+    plan.begins[b] = 0;
+  }
   auto keys_of = [&](int b) { return b < LENS_HELD ? plan.lens[b] : clamped(l.kv_lens[b], 0, l.most); };
   for (int g = lane; g < l.num_groups; g += 64) {
     const int start = clamped(g < 64 ? start0 : l.group_starts[g], 0, l.num_seqs), end = clamped(g < 64 ? end0 : l.group_starts[g + 1], start, l.num_seqs);
     plan.start[g] = start;
     plan.end[g] = end;
     plan.shared[g] = end - start > 1 ? clamped(g < 64 ? shared0 : l.shared_lens[g], 0, keys_of(start)) : 0;
+    if (end > start && start < LENS_HELD) plan.begins[start] = g + 1;
   }
   struct Own { int group, from, to; };  // a sequence's own keys [from, to); group: whose shared keys it has, or -1
-  auto own_of = [&](int b) {
-    const int len = keys_of(b);
-    int lo = -1, hi = l.num_groups;  // the last group that begins at b or before
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (plan.start[mid] <= b) lo = mid;
-      else hi = mid;
+  // of sequence base + lane; `latest` is 1 + the last group that begins before `base`, or 0, and on return before base + 64
+  auto own_of = [&](int base, int& latest) {
+    const int b = base + lane;
+    int group = 0;
+    if (base + 64 <= LENS_HELD) {
+      group = max(most_up_to_lane(b < l.num_seqs ? plan.begins[b] : 0), latest);
+      latest = __builtin_amdgcn_readlane(group, 63);
+    } else {
+      int lo = -1, hi = l.num_groups;  // the last group that begins at b or before
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (plan.start[mid] <= b) lo = mid;
+        else hi = mid;
+      }
+      group = lo + 1;
     }
-    const int shared = lo >= 0 && b < plan.end[lo] ? plan.shared[lo] : 0;
-    return shared > 0 && shared <= len ? Own{lo, shared, len} : Own{-1, 0, len};
+    if (b >= l.num_seqs) return Own{-1, 0, 0};
+    const int len = keys_of(b), shared = group > 0 && b < plan.end[group - 1] ? plan.shared[group - 1] : 0;
+    return shared > 0 && shared <= len ? Own{group - 1, shared, len} : Own{-1, 0, len};
   };
   auto blocks_of = [&](int g) { return plan.shared[g] > 0 ? ((plan.end[g] - plan.start[g]) * l.group + l.block_rows - 1) >> block_shift : 0; };
   auto steps_of = [&](int keys) { return (unsigned)(keys + STEP - 1) / STEP; };
   auto tiles_of = [&](const Own& own) { return own.to > own.from ? (int)((unsigned)(own.to + TILE - 1) / TILE - (unsigned)own.from / TILE) : 0; };
   // steps of all items, and how many one may have
-  const Own own0 = lane < l.num_seqs ? own_of(lane) : Own{-1, 0, 0};
-  int steps = 0, tiles = lane < l.num_seqs ? own_blocks * tiles_of(own0) : 0;
+  int latest = 0;
+  const Own own0 = own_of(0, latest);
+  const int latest0 = latest;
+  int steps = 0, tiles = own_blocks * tiles_of(own0);
   for (int g = lane; g < l.num_groups; g += 64) steps += blocks_of(g) * steps_of(plan.shared[g]);
-  for (int b = 64 + lane; b < l.num_seqs; b += 64) tiles += own_blocks * tiles_of(own_of(b));
+  for (int base = 64; base < l.num_seqs; base += 64) tiles += own_blocks * tiles_of(own_of(base, latest));
   steps = __builtin_amdgcn_readlane(sum_up_to_lane(steps), 63);
   tiles = __builtin_amdgcn_readlane(sum_up_to_lane(tiles), 63);
   const int per = max(1, (steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target);
@@ -202,9 +232,10 @@ __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) 
   // the sequences' items; every sequence has one at least, which writes down where its rows lie
   const int item = (wg - group_items) * WAVES + wave;
   before = 0;
+  latest = latest0;
   for (int base = 0; base < l.num_seqs; base += 64) {
     const int b = base + lane;
-    const Own own = base == 0 ? own0 : b < l.num_seqs ? own_of(b) : Own{-1, 0, 0};
+    const Own own = base == 0 ? own0 : own_of(base, latest);
     const int parts = max(1, parts_of(tiles_of(own), per)), items = b < l.num_seqs ? own_blocks * parts : 0;
     const int upto = before + sum_up_to_lane(items);
     const uint64_t holds = __ballot(upto > item);
@@ -699,20 +730,24 @@ __global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int
   for (int p0 = 0; p0 < parts; p0 += 64) {
     const int here = min(parts - p0, 64);
     const float log_sum = lane < here ? part_lse[place_of(p0 + lane)] : -INFINITY;
-    channels_t o[AHEAD];
+    auto join = [&](auto ahead) {
+      constexpr int N = decltype(ahead)::value;
+      channels_t o[N];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      o[j] = *reinterpret_cast<const channels_t*>(channels + place_of(p0 + (j < here ? j : here - 1)) * D);  // (no branch, or each would wait for the one before)
-    const float now = fmaxf(top, wave_max(log_sum)), safe = now == -INFINITY ? 0.f : now, old = top == -INFINITY ? 0.f : expf(top - safe);
-    const float weight = log_sum == -INFINITY ? 0.f : expf(log_sum - safe);
-    denom = denom * old + wave_sum(weight);
-    acc = acc * old;
-    top = now;
-    auto weight_of = [&](int j) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), j)); };
+      for (int j = 0; j < N; ++j)
+        o[j] = *reinterpret_cast<const channels_t*>(channels + place_of(p0 + (j < here ? j : here - 1)) * D);  // (no branch, or each would wait for the one before)
+      const float now = fmaxf(top, wave_max(log_sum)), safe = now == -INFINITY ? 0.f : now, old = top == -INFINITY ? 0.f : expf(top - safe);
+      const float weight = log_sum == -INFINITY ? 0.f : expf(log_sum - safe);
+      denom = denom * old + wave_sum(weight);
+      acc = acc * old;
+      top = now;
+      auto weight_of = [&](int j) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), j)); };
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      acc += (j < here ? o[j] : channels_t(0.f)) * weight_of(j);  // (a part without a key holds zeros)
-    for (int j = AHEAD; j < here; ++j) acc += *reinterpret_cast<const channels_t*>(channels + place_of(p0 + j) * D) * weight_of(j);
+      for (int j = 0; j < N; ++j) acc += (j < here ? o[j] : channels_t(0.f)) * weight_of(j);  // (a part without a key holds zeros)
+      for (int j = N; j < here; ++j) acc += *reinterpret_cast<const channels_t*>(channels + place_of(p0 + j) * D) * weight_of(j);
+    };
+    if (here <= 6) join(std::integral_constant<int, 6>{});
+    else join(std::integral_constant<int, AHEAD>{});
   }
   if (sinks != nullptr && top != -INFINITY) denom += expf(sinks[head] - top);
   if (!live) return;

@@ -12,8 +12,10 @@ behind ``torch.nn.functional.linear`` (hipBLASLt) where ``HipOps.linear`` says s
 """
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
+import functools
 import logging
 import os
 import tempfile
@@ -109,6 +111,7 @@ class HipOps:
         self._shared_prefix: Dict[int, ctypes.CDLL] = {}
         self._beams: Optional[ctypes.CDLL] = None
         self._declare_core()
+        self._index = self.device.index
         self.num_cus = torch.cuda.get_device_properties(self.device).multi_processor_count
         self.use_library_gemm = True
         self.use_skinny_gemm = True
@@ -411,9 +414,23 @@ class HipOps:
             return _P(self._raw_stream(self.device.index))
         return _P(torch.cuda.current_stream(self.device).cuda_stream)
 
-    def _current(self):
-        """The kernels' device as the current one (a launch goes to the current device's queues)."""
-        return contextlib.nullcontext() if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
+    def _take(self, name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int, ...], align: int = 4) -> int:
+        """A tensor's address, after ``_check``'s checks (which speak where one fails)."""
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._index or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+            self._check(name, t, dtype, shape, align)
+        address = t.data_ptr()
+        if address % align != 0:
+            self._check(name, t, dtype, shape, align)
+        return address
+
+    def _call(self, what: str, function, *args) -> None:
+        """Launches with the kernels' device as the current one (a launch goes to the current device's queues)."""
+        if torch._C._cuda_getDevice() == self._index:
+            status = function(*args, self._stream())
+        else:
+            with torch.cuda.device(self.device):
+                status = function(*args, self._stream())
+        self._launched(status, what)
 
     def _check(self, name: str, t: torch.Tensor, dtype=None, shape=None, align: int = 4) -> None:
         if not isinstance(t, torch.Tensor) or t.device != self.device:
@@ -2301,7 +2318,9 @@ class HipOps:
     MAX_BEAMS, MAX_KEPT, MAX_BEAM_VOCAB = 256, 64, 1 << 24  # of ``beam_select``
     MAX_MOVED = 64  # beams of a request that ``reorder_states`` moves
 
-    def _shared_prefix_shape(self, num_seqs: int, num_groups: int, num_heads: int, num_kv_heads: int, head_dim: int, element_size: int, largest_group: int) -> Tuple[int, int, int, int]:
+    @staticmethod
+    @functools.lru_cache(maxsize=4096)
+    def _shared_prefix_shape(num_cus: int, num_seqs: int, num_groups: int, num_heads: int, num_kv_heads: int, head_dim: int, element_size: int, largest_group: int) -> Tuple[int, int, int, int]:
         """Row tiles of a workgroup, over how many workgroups per KV head the keys are cut, and how many workgroups and rows of partial results
         per KV head that makes at most (as ``velox_shared_prefix_room`` counts them)."""
         group = num_heads // num_kv_heads
@@ -2311,19 +2330,21 @@ class HipOps:
             row_tiles *= 2
         if element_size == 2 and head_dim in (64, 128) and largest_group * group > 64:
             row_tiles = 8
-        target = max(1, 2 * self.num_cus // num_kv_heads)
+        # A workgroup per compute unit, two of the kernel for many rows.  Measured on MI355X (us, one / two): 8 groups of 4 behind 1,024 to 2,048 keys, 28 heads over 4,
+        # 12.6 + 4.2 and 13.8 + 12.2 (of which the second joins the parts), 5 of 8 in float32 15.8 and 21.4; 64 behind 8,192 keys 35.5 and 27.1, behind 32,768 161 and 109.
+        target = max(1, (2 if row_tiles == 8 else 1) * num_cus // num_kv_heads)
         own_blocks, blocks = num_seqs * (-(-group // 16)), num_seqs * group // (16 * row_tiles) + num_groups
         return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(16 * row_tiles, 64) + blocks * 16 * row_tiles + own_blocks * 16 + 64
 
-    def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> Tuple[int, int]:
-        """The most float32 elements ``shared_prefix_attention`` asks its workspace for (``shared_prefix_out``, ``shared_prefix_lse``) in any
-        step of at most so many sequences and groups, whatever the lengths and the element type."""
+    def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> int:
+        """The most float32 elements ``shared_prefix_attention`` asks its workspace for (``shared_prefix_parts``) in any step of at most so many
+        sequences and groups, whatever the lengths and the element type."""
         rows = 0
         for element_size in (2, 4):
             for largest in (1, 1 << 20):
                 for groups in (0, max_num_groups):
-                    rows = max(rows, self._shared_prefix_shape(max_num_seqs, groups, num_heads, num_kv_heads, head_dim, element_size, largest)[3])
-        return rows * num_kv_heads * head_dim, rows * num_kv_heads + 8 * max_num_seqs
+                    rows = max(rows, self._shared_prefix_shape(self.num_cus, max_num_seqs, groups, num_heads, num_kv_heads, head_dim, element_size, largest)[3])
+        return rows * num_kv_heads * (head_dim + 1) + 8 * max_num_seqs
 
     def shared_prefix_attention(self, qkv, num_heads, num_kv_heads, head_dim, k_cache, v_cache, block_size, block_tables, kv_lens, group_starts, shared_lens,
                                 largest_group, max_kv_len, scale, workspace, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2338,57 +2359,53 @@ class HipOps:
         ``largest_group``: sequences of the largest group (which kernel is launched goes by it, the result does not), ``max_kv_len``: the most keys
         of any sequence (a greater length counts as that many).  Lengths and groups are read on the device only: a captured call replays with other ones, as long as the number of
         sequences and groups stays.  ``sinks``: as for ``paged_attention``.  Pages hold at least 8 tokens."""
-        num_seqs = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-        width = qkv.shape[1] if qkv.dim() == 2 else -1
+        num_seqs, num_groups = kv_lens.numel(), shared_lens.numel()
+        dtype = qkv.dtype
+        element_size = 2 if dtype == torch.bfloat16 else 4
         if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads != 0:
             raise KernelError("num_heads must be a multiple of num_kv_heads")
         if head_dim % 16 != 0 or not 16 <= head_dim <= self.MAX_TILED_HEAD_DIM:
             raise KernelError(f"shared_prefix_attention: head_dim={head_dim} is no multiple of 16 up to {self.MAX_TILED_HEAD_DIM}")
-        if width not in (num_heads * head_dim, (num_heads + 2 * num_kv_heads) * head_dim):
+        width = qkv.shape[1] if qkv.dim() == 2 else -1
+        if width != num_heads * head_dim and width != (num_heads + 2 * num_kv_heads) * head_dim:
             raise KernelError(f"shared_prefix_attention: rows of {width} elements hold neither the queries nor queries, keys and values")
-        dtype = _code(qkv.dtype)
-        self._check("kv_lens", kv_lens, torch.int32, (num_seqs,))
-        self._check("qkv", qkv, None, (num_seqs, width), align=16)
-        self._check("group_starts", group_starts, torch.int32)
-        self._check("shared_lens", shared_lens, torch.int32)
-        num_groups = shared_lens.numel()
-        if shared_lens.dim() != 1 or tuple(group_starts.shape) != (num_groups + 1,) or num_groups > self.MAX_PREFIX_GROUPS:
-            raise KernelError(f"shared_prefix_attention: {tuple(group_starts.shape)} starts do not go with {tuple(shared_lens.shape)} groups, at most {self.MAX_PREFIX_GROUPS}")
-        self._check("block_tables", block_tables, torch.int32)
-        if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs:
-            raise KernelError(f"block_tables must be [{num_seqs}, W], got {tuple(block_tables.shape)}")
+        if num_groups > self.MAX_PREFIX_GROUPS:
+            raise KernelError(f"shared_prefix_attention: {num_groups} groups, at most {self.MAX_PREFIX_GROUPS} are taken")
+        code = _code(dtype)
+        qkv_at = self._take("qkv", qkv, dtype, (num_seqs, width), 16)
+        lens_at = self._take("kv_lens", kv_lens, torch.int32, (num_seqs,))
+        shared_at = self._take("shared_lens", shared_lens, torch.int32, (num_groups,))
+        starts_at = self._take("group_starts", group_starts, torch.int32, (num_groups + 1,))
+        table_width = block_tables.shape[1] if block_tables.dim() == 2 else 0
+        tables_at = self._take("block_tables", block_tables, torch.int32, (num_seqs, table_width))
         if block_size < 8 or block_size & (block_size - 1):
             raise KernelError(f"shared_prefix_attention: block_size must be a power of two from 8 on, got {block_size}")
-        if max_kv_len < 0 or block_tables.shape[1] * block_size < max_kv_len:
-            raise KernelError(f"block tables of width {block_tables.shape[1]} cannot cover {max_kv_len} keys")
+        if max_kv_len < 0 or table_width * block_size < max_kv_len:
+            raise KernelError(f"block tables of width {table_width} cannot cover {max_kv_len} keys")
         pages = k_cache.shape[0]
         if pages < 1:
             raise KernelError("shared_prefix_attention: a cache without pages")
-        self._check("k_cache", k_cache, qkv.dtype, (pages, num_kv_heads, block_size, head_dim), align=16)
-        self._check("v_cache", v_cache, qkv.dtype, (pages, num_kv_heads, head_dim, block_size), align=16)
+        keys_at = self._take("k_cache", k_cache, dtype, (pages, num_kv_heads, block_size, head_dim), 16)
+        values_at = self._take("v_cache", v_cache, dtype, (pages, num_kv_heads, head_dim, block_size), 16)
         if not 0 < scale < float("inf"):
             raise KernelError(f"shared_prefix_attention: the scale must be positive, got {scale}")
-        if sinks is not None:
-            self._check("sinks", sinks, torch.float32, (num_heads,))
+        sinks_at = 0 if sinks is None else self._take("sinks", sinks, torch.float32, (num_heads,))
         if not 1 <= largest_group <= max(num_seqs, 1):
             raise KernelError(f"shared_prefix_attention: a largest group of {largest_group} among {num_seqs} sequences")
         if workspace is None:
             raise KernelError("shared_prefix_attention needs a workspace")
-        out = torch.empty((num_seqs, num_heads * head_dim), dtype=qkv.dtype, device=self.device)
+        out = torch.empty((num_seqs, num_heads * head_dim), dtype=dtype, device=self.device)
         if num_seqs == 0:
             return out
-        row_tiles, target, items, rows = self._shared_prefix_shape(num_seqs, num_groups, num_heads, num_kv_heads, head_dim, qkv.element_size(), int(largest_group))
+        row_tiles, target, items, rows = self._shared_prefix_shape(self.num_cus, num_seqs, num_groups, num_heads, num_kv_heads, head_dim, element_size, int(largest_group))
         if items > 65535 or num_seqs > 65535:
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
-        part_o = workspace.get("shared_prefix_out", rows * num_kv_heads * head_dim)
-        part_lse = workspace.get("shared_prefix_lse", rows * num_kv_heads + 8 * num_seqs)  # (and where the sequences' rows lie, eight numbers each)
-        lib = self.shared_prefix_library(head_dim)
-        with self._current():
-            status = lib.velox_shared_prefix_attention(
-                _ptr(qkv), width, _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), block_tables.shape[1], _ptr(kv_lens), _ptr(group_starts), _ptr(shared_lens), num_seqs,
-                num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages, int(max_kv_len), float(scale), row_tiles, target, items, rows, _ptr(sinks), _ptr(out),
-                _ptr(part_o), _ptr(part_lse), _ptr(part_lse[rows * num_kv_heads:]), dtype, self._stream())
-        self._launched(status, "shared_prefix_attention")
+        # partial outputs, their log-sums, and where each sequence's rows of them lie, eight numbers
+        rows_all = rows * num_kv_heads
+        parts = workspace.get("shared_prefix_parts", rows_all * (head_dim + 1) + 8 * num_seqs).data_ptr()
+        self._call("shared_prefix_attention", self.shared_prefix_library(head_dim).velox_shared_prefix_attention, qkv_at, width, keys_at, values_at, tables_at, table_width,
+                   lens_at, starts_at, shared_at, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages, int(max_kv_len), float(scale), row_tiles,
+                   target, items, rows, sinks_at, out.data_ptr(), parts, parts + 4 * rows_all * head_dim, parts + 4 * rows_all * (head_dim + 1), code)
         return out
 
     def _beam_pieces(self, rows: int, vocab: int) -> int:
@@ -2403,31 +2420,29 @@ class HipOps:
         by token ``v`` is worth ``scores[w] + log_softmax(logits[w])[v]``, in 64 bits.  Returns, best first, their values (float32), their beams
         and their tokens (int32), each ``[requests, keep]``.  Equal ones come by the lowest beam, then by the greater logit, then by the lowest token;
         a logit that is -inf or no number makes a value of -inf, and those come last."""
-        self._check("logits", logits, torch.float32)
-        self._check("scores", scores, torch.float32)
         if logits.dim() != 2 or scores.dim() != 2 or scores.numel() != logits.shape[0]:
             raise KernelError(f"beam_select: {tuple(scores.shape)} scores do not go with logits of shape {tuple(logits.shape)}")
-        (requests, beams), vocab, keep = scores.shape, logits.shape[1], int(keep)
+        (requests, beams), (rows, vocab), keep = scores.shape, logits.shape, int(keep)
+        logits_at = self._take("logits", logits, torch.float32, (rows, vocab))
+        scores_at = self._take("scores", scores, torch.float32, (requests, beams))
         if not 1 <= beams <= self.MAX_BEAMS or not 1 <= vocab <= self.MAX_BEAM_VOCAB:
             raise KernelError(f"beam_select: {beams} beams over {vocab} tokens; 1 to {self.MAX_BEAMS} and 1 to {self.MAX_BEAM_VOCAB} are taken")
         if not 1 <= keep <= min(self.MAX_KEPT, beams * vocab):
             raise KernelError(f"beam_select: keep={keep} is not between 1 and {min(self.MAX_KEPT, beams * vocab)}")
-        rows = requests * beams
         if rows > 65535:
             raise KernelError(f"beam_select: {rows} rows exceed the launch grid")
-        values = torch.empty((requests, keep), dtype=torch.float32, device=self.device)
-        parents = torch.empty((requests, keep), dtype=torch.int32, device=self.device)
-        tokens = torch.empty((requests, keep), dtype=torch.int32, device=self.device)
+        device = self.device
+        values = torch.empty((requests, keep), dtype=torch.float32, device=device)
+        parents = torch.empty((requests, keep), dtype=torch.int32, device=device)
+        tokens = torch.empty((requests, keep), dtype=torch.int32, device=device)
         if requests == 0:
             return values, parents, tokens
         lib = self.beam_library()
         pieces = self._beam_pieces(rows, vocab)
-        size = int(lib.velox_beam_scratch_bytes(rows, pieces, keep))
-        scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
-        with self._current():
-            status = lib.velox_beam_select(_ptr(logits), _ptr(scores), requests, beams, vocab, keep, pieces, _ptr(scratch), size, _ptr(values), _ptr(parents), _ptr(tokens),
-                                           self._stream())
-        self._launched(status, "beam_select")
+        size = lib.velox_beam_scratch_bytes(rows, pieces, keep)
+        scratch = torch.empty(size, dtype=torch.uint8, device=device)
+        self._call("beam_select", lib.velox_beam_select, logits_at, scores_at, requests, beams, vocab, keep, pieces, scratch.data_ptr(), size, values.data_ptr(),
+                   parents.data_ptr(), tokens.data_ptr())
         return values, parents, tokens
 
     def reorder_states(self, tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents: torch.Tensor, axis: int = 0) -> None:
@@ -2435,47 +2450,45 @@ class HipOps:
         ``slots[b, parents[b, j], p]`` was before the call.  ``slots`` int32 ``[requests, beams]`` or ``[requests, beams, rows]`` (state slots, or the pages behind
         a shared prefix), ``parents`` int32 ``[requests, beams]``, at most ``MAX_MOVED`` beams.  A row or a parent outside its range (-1: none) moves nothing
         and is not moved to.  Every row belongs to one beam of one request, and the tensors share no memory."""
-        self._check("slots", slots, torch.int32)
-        self._check("parents", parents, torch.int32)
         if parents.dim() != 2 or slots.dim() not in (2, 3) or slots.shape[:2] != parents.shape:
             raise KernelError(f"reorder_states: slots of shape {tuple(slots.shape)} do not go with parents of shape {tuple(parents.shape)}")
         requests, beams = parents.shape
         places = slots.shape[2] if slots.dim() == 3 else 1
+        slots_at, parents_at = self._take("slots", slots, torch.int32, slots.shape), self._take("parents", parents, torch.int32, parents.shape)
         if not 1 <= beams <= self.MAX_MOVED or requests * places > 65535:
             raise KernelError(f"reorder_states: {requests} requests of {beams} beams with {places} rows; 1 to {self.MAX_MOVED} beams and 65,535 rows of a beam are taken")
-        described, spans = [], []
+        described = []
         for at, t in enumerate(tensors):
-            self._check(f"tensors[{at}]", t, align=1)
-            if not 0 <= axis < t.dim():
-                raise KernelError(f"reorder_states: tensors[{at}] of shape {tuple(t.shape)} has no dimension {axis}")
-            if t.numel() == 0:
+            start = self._take(f"tensors[{at}]", t, t.dtype, t.shape, 1)
+            shape = t.shape
+            if not 0 <= axis < len(shape):
+                raise KernelError(f"reorder_states: tensors[{at}] of shape {tuple(shape)} has no dimension {axis}")
+            count = t.numel()
+            if count == 0:
                 continue
-            outer, rows = 1, t.shape[axis]
-            for n in t.shape[:axis]:
+            outer = 1
+            for n in shape[:axis]:
                 outer *= n
-            run = t.numel() // outer * t.element_size()
+            rows, run = shape[axis], count // outer * t.element_size()
             if outer > 65535 or rows > 0x7FFFFFFF:
-                raise KernelError(f"reorder_states: tensors[{at}] of shape {tuple(t.shape)} exceeds the launch grid")
-            start = t.data_ptr()
+                raise KernelError(f"reorder_states: tensors[{at}] of shape {tuple(shape)} exceeds the launch grid")
             described.append((start, outer, run, rows, run // rows))
-            spans.append((start, start + outer * run))
-        spans.sort()
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise KernelError("reorder_states: two tensors share memory")
+        if len(described) > 1:
+            in_order = sorted(described)
+            if any(a[0] + a[1] * a[2] > b[0] for a, b in zip(in_order, in_order[1:])):
+                raise KernelError("reorder_states: two tensors share memory")
         if requests * places == 0 or not described:
             return
-        lib = self.beam_library()
+        launch = self.beam_library().velox_reorder_states
         at = 0
-        with self._current():
-            while at < len(described):  # up to 32 tensors and 65,535 runs of rows a launch
-                end, runs = at, 0
-                while end < len(described) and end - at < 32 and runs + described[end][1] <= 65535:
-                    runs += described[end][1]
-                    end += 1
-                numbers = [n for d in described[at:end] for n in d]
-                status = lib.velox_reorder_states((ctypes.c_longlong * len(numbers))(*numbers), end - at, _ptr(slots), _ptr(parents), requests, beams, places, self._stream())
-                self._launched(status, "reorder_states")
-                at = end
+        while at < len(described):  # up to 32 tensors and 65,535 runs of rows a launch
+            end, runs = at, 0
+            while end < len(described) and end - at < 32 and runs + described[end][1] <= 65535:
+                runs += described[end][1]
+                end += 1
+            numbers = array.array("q", [n for d in described[at:end] for n in d])
+            self._call("reorder_states", launch, numbers.buffer_info()[0], end - at, slots_at, parents_at, requests, beams, places)
+            at = end
 
     # -- sampling -------------------------------------------------------------------------------
     def argmax(self, logits: torch.Tensor) -> torch.Tensor:
