@@ -152,6 +152,28 @@ def test_attention_long(ops, workspace, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim,count,shared", [(28, 4, 128, 20, 2048), (10, 2, 128, 64, 1500), (28, 4, 64, 40, 3001), (8, 1, 128, 17, 8192)])
+def test_attention_many_rows(ops, workspace, dtype, heads, kv_heads, dim, count, shared):
+    """Several blocks of many rows over many tiles, the last block in part; the same bits every time."""
+    b = Batch(dtype, heads, kv_heads, dim, 16, groups=[(count, shared), (2, 100)], lens=own(count, shared, 1, 150) + [120, 101], seed=count)
+    first = b.run(ops, workspace)
+    b.check(first)
+    for _ in range(50):
+        assert torch.equal(first, b.run(ops, workspace))
+
+
+def test_attention_more_sequences_than_are_held(ops, workspace):
+    """More than 1,024 sequences, in groups and not."""
+    groups = [(1 + g % 4, 5 + g % 60) for g in range(520)]
+    lens = [s + 1 + (i % 3) for i, s in enumerate(s for c, s in groups for _ in range(c))]
+    b = Batch(BF16, 2, 1, 16, 8, groups=groups, lens=lens + [7] * 20, behind=20)
+    first = b.run(ops, workspace)
+    b.check(first)
+    for _ in range(10):
+        assert torch.equal(first, b.run(ops, workspace))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_attention_many_sequences_and_groups(ops, workspace, dtype):
     """More than 64 of both (a wave's lanes), most of them short."""
     groups = [(1 + g % 3, 9 + g) for g in range(70)]

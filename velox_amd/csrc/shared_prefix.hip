@@ -142,8 +142,8 @@ __device__ __forceinline__ int sum_up_to_lane(int v) {
   return v;
 }
 
-// The item of workgroup `wg`, and in it of this wave.  Every wave works it out for itself (all write the same to `plan`, and each reads what
-// it has written), with no barrier: a lane has a group and a sequence of its own, 64 of each at a time.
+// The item of workgroup `wg`, and in it of this wave.  Every wave works it out for itself: a lane has a group and a sequence of its own, 64 of
+// each at a time; all waves write the same to `plan`, each reads what it has written itself, and the one barrier is behind the zeros that are written first.
 template <int TILE>
 __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) {
   constexpr int STEP = WAVES * TILE;
@@ -159,10 +159,9 @@ __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) 
     shared0 = l.shared_lens[g];
   }
   const int len0 = l.kv_lens[at_most(lane, l.num_seqs)];
-  for (int b = lane; b < l.num_seqs && b < LENS_HELD; b += 64) {
-    plan.lens[b] = clamped(b < 64 ? len0 : l.kv_lens[b], 0, l.most);
-    plan.begins[b] = 0;
-  }
+  for (int b = threadIdx.x; b < l.num_seqs && b < LENS_HELD; b += THREADS) plan.begins[b] = 0;
+  __syncthreads();
+  for (int b = lane; b < l.num_seqs && b < LENS_HELD; b += 64) plan.lens[b] = clamped(b < 64 ? len0 : l.kv_lens[b], 0, l.most);
   auto keys_of = [&](int b) { return b < LENS_HELD ? plan.lens[b] : clamped(l.kv_lens[b], 0, l.most); };
   for (int g = lane; g < l.num_groups; g += 64) {
     const int start = clamped(g < 64 ? start0 : l.group_starts[g], 0, l.num_seqs), end = clamped(g < 64 ? end0 : l.group_starts[g + 1], start, l.num_seqs);
@@ -204,7 +203,16 @@ __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) 
   for (int base = 64; base < l.num_seqs; base += 64) tiles += own_blocks * tiles_of(own_of(base, latest));
   steps = __builtin_amdgcn_readlane(sum_up_to_lane(steps), 63);
   tiles = __builtin_amdgcn_readlane(sum_up_to_lane(tiles), 63);
-  const int per = max(1, (steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target);
+  int per = max(1, (steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target);
+  if (l.block_rows > 16 * WAVES) {
+    // (many rows: `target` workgroups fill the compute units, and the first one more would be a whole round; rounding parts up can bring it about)
+    for (int tries = 0; tries < 6; ++tries) {
+      int items = 0;
+      for (int g = lane; g < l.num_groups; g += 64) items += blocks_of(g) * parts_of(steps_of(plan.shared[g]), per);
+      if (__builtin_amdgcn_readlane(sum_up_to_lane(items), 63) <= l.target) break;
+      per += 1 + (per >> 4);
+    }
+  }
   // the groups' items
   Item found = {-1, -1, 0, 0, 0, 0, 0, 0, false, {}};
   int before = 0;
@@ -489,6 +497,7 @@ __device__ __forceinline__ void join_waves(Rows<T, RT>& rows, int count, float* 
 }
 
 // ---- many rows: tiles in LDS ------------------------------------------------------------------------------------------------------
+// `idle`: the wave has no rows and only brings tiles.
 // From some hundred rows on the products count, and every 32 rows reading the keys for themselves is more than the second-level caches give.  Here the four
 // waves have 32 rows each and share tiles of 64 keys (bfloat16, heads of 64 and 128 channels).  Every lane asks for 16 bytes of the cache with a
 // load that writes LDS itself, a whole tile ahead of the one being multiplied, into the other of two buffers; one barrier a tile is left.  Such a load fills
@@ -498,7 +507,7 @@ __device__ __forceinline__ void join_waves(Rows<T, RT>& rows, int count, float* 
 constexpr int TALL_TILE = 64, TALL_ROWS = 32 * WAVES;
 constexpr bool HAS_TALL = D == 64 || D == 128;
 constexpr int TALL_BYTES = TALL_TILE * D * 2;  // of the keys or the values of a tile
-__device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf16_t>& cache, int kvh, const int* __restrict__ table, int lo, int hi, float scale,
+__device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf16_t>& cache, int kvh, const int* __restrict__ table, int lo, int hi, float scale, bool idle,
                                           char (*smem)[2 * TALL_BYTES]) {
   typedef Block<bf16_t> B;
   constexpr int CT = 2, NQB = Rows<bf16_t, 2>::NQB, NC = D / 16, NT = TALL_TILE / 16, NKB = TALL_TILE / 32;
@@ -516,8 +525,9 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
   const uint32_t value_elems = (uint32_t)(kvh * D + 8 * wave + (lane >> 3)) << cache.page_shift;
   // lane e's page id, e < 8, is that of the tile's keys 8 e .. 8 e + 7, or of the last keys there are
   auto load_id = [&](int n0) { return min((uint32_t)table[min(n0 + 8 * (lane & 7), hi - 1) >> cache.page_shift], cache.last_page); };
-  auto issue = [&](int n0, uint32_t id, char* to) {
+  auto issue_keys = [&](int n0, uint32_t id, int buffer) {
     const int at = __builtin_amdgcn_readfirstlane(n0);
+    char* const to = smem[__builtin_amdgcn_readfirstlane(buffer)];
 #pragma unroll
     for (int m = 0; m < LOADS; ++m) {
       const int key0 = KEYS * (wave + WAVES * m);
@@ -525,10 +535,14 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
       const bf16_t* base = cache.k + (((page * cache.nkv + kvh) << cache.page_shift) + ((at + key0) & (page_size - 1))) * D;
       load_to_lds_16(base, key_bytes, to + 1024 * (wave + WAVES * m));
     }
+  };
+  auto issue_values = [&](int n0, uint32_t id, int buffer) {
+    const int at = __builtin_amdgcn_readfirstlane(n0);
+    char* const to = smem[__builtin_amdgcn_readfirstlane(buffer)] + TALL_BYTES;
     const uint32_t page = __shfl(id, value_eight, VELOX_WAVE);
     const bf16_t* from = cache.v + (size_t)page * page_elems + (value_elems + (uint32_t)((at + 8 * value_eight) & (page_size - 1)));
 #pragma unroll
-    for (int m = 0; m < LOADS; ++m) load_to_lds_16(from + ((size_t)(8 * WAVES * m) << cache.page_shift), to + TALL_BYTES + 1024 * (wave + WAVES * m));
+    for (int m = 0; m < LOADS; ++m) load_to_lds_16(from + ((size_t)(8 * WAVES * m) << cache.page_shift), to + 1024 * (wave + WAVES * m));
   };
   // where each lane reads its operands: row 8 (i / 4) + i % 4 of a block of 32 keys (+ 4 u for score tile u), pieces 4 cb + g; row i of a channel tile,
   // pieces 4 kb + g
@@ -538,23 +552,7 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
   const int value_first = value_row + 64 * half, value_second = value_row + 64 * (1 - half);
   const float scale_eff = scale * B::SCALE;
 
-  // (the queries have arrived before the loop, said in a way the compiler sees: it would otherwise wait for them, and with them for every
-  // load in flight, in every round)
-  uint32_t id = load_id(lo), next_id = load_id(lo + TALL_TILE);
-  __builtin_amdgcn_s_waitcnt(0x0F70);
-  issue(lo, id, smem[0]);
-  int buffer = 0;
-  for (int n0 = lo; n0 < hi; n0 += TALL_TILE, buffer ^= 1) {
-    wait_for_loads<0>();  // this wave's pieces of the tile have landed
-    __syncthreads();      // everybody's have, and everybody is done with the other buffer
-    if (n0 + TALL_TILE < hi) {
-      id = next_id;
-      next_id = load_id(n0 + 2 * TALL_TILE);
-      issue(n0 + TALL_TILE, id, smem[buffer ^ 1]);
-    }
-    const char* const tile = smem[buffer];
-    const bool whole = n0 + TALL_TILE <= hi;
-    float4_t s[CT][NT];
+  auto multiply_keys = [&](float4_t (&s)[CT][NT], const char* tile) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float4_t k[NQB];
@@ -568,17 +566,45 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) s[ct][t] = B::mma(k[cb], rows.q[ct][cb], s[ct][t]);
     }
+  };
+  // A tile's keys are asked for two tiles ahead of its values' product and its values one: while the weights of a tile are worked out from their
+  // scores, the next tile's scores are already being multiplied.
+  uint32_t id = load_id(lo), next_id = load_id(lo + TALL_TILE), far_id = load_id(lo + 2 * TALL_TILE);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // (the queries have arrived, said in a way the compiler sees: it would otherwise wait in every round)
+  issue_keys(lo, id, 0);
+  wait_for_loads<0>();
+  __syncthreads();
+  issue_values(lo, id, 0);
+  if (lo + TALL_TILE < hi) issue_keys(lo + TALL_TILE, next_id, 1);
+  float4_t s0[CT][NT], s1[CT][NT];
+  if (!idle) multiply_keys(s0, smem[0]);
+  auto round = [&](float4_t (&s)[CT][NT], float4_t (&next)[CT][NT], int n0, int buffer) {
+    wait_for_loads<0>();  // this wave's pieces of this tile's values and the next one's keys have landed
+    __syncthreads();      // everybody's have, and everybody is done with the buffers that are filled now
+    id = next_id;
+    next_id = far_id;
+    far_id = load_id(n0 + 3 * TALL_TILE);
+    if (n0 + TALL_TILE < hi) issue_values(n0 + TALL_TILE, id, buffer ^ 1);
+    if (n0 + 2 * TALL_TILE < hi) issue_keys(n0 + 2 * TALL_TILE, next_id, buffer);
+    if (idle) return;
+    const bool whole = n0 + TALL_TILE <= hi;
+    if (!whole) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[ct][t][j] = n0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + j < hi ? s[ct][t][j] : -INFINITY;
+    }
+    // (matrix instructions first: the other wave of the SIMD then has the vector unit for its weights meanwhile)
+    __builtin_amdgcn_s_setprio(1);
+    multiply_keys(next, smem[buffer ^ 1]);  // (behind the last tile: of whatever lies there, and not used)
+    __builtin_amdgcn_s_setprio(0);
     float alpha[CT];
     float4_t pf[CT][NKB];
     bool moved = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      if (!whole) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[ct][t][j] = n0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + j < hi ? s[ct][t][j] : -INFINITY;
-      }
       float mx = -INFINITY;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -615,24 +641,26 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = rows.acc[ct][c] * alpha[ct];
     }
-    float4_t v[2][NKB];  // a channel tile's operands are in flight ahead of the one being multiplied
-    auto read_values = [&](int c, float4_t (&into)[NKB]) {
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        into[kb] = *reinterpret_cast<const float4_t*>(tile + (kb ? value_second : value_first) + 2048 * c);
-        if (!whole) B::mask(into[kb], 0, hi - (n0 + 32 * kb + 8 * g));
-      }
-    };
-    read_values(0, v[0]);
+    __builtin_amdgcn_s_setprio(1);
+    const char* const tile = smem[buffer];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (c + 1 < NC) read_values(c + 1, v[(c + 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);
+      float4_t v[NKB];
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        v[kb] = *reinterpret_cast<const float4_t*>(tile + (kb ? value_second : value_first) + 2048 * c);
+        if (!whole) B::mask(v[kb], 0, hi - (n0 + 32 * kb + 8 * g));
+      }
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = B::mma(v[c & 1][kb], pf[ct][kb], rows.acc[ct][c]);
+        for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = B::mma(v[kb], pf[ct][kb], rows.acc[ct][c]);
     }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  for (int n0 = lo; n0 < hi; n0 += 2 * TALL_TILE) {
+    round(s0, s1, n0, 0);
+    if (n0 + TALL_TILE < hi) round(s1, s0, n0 + TALL_TILE, 1);
   }
 }
 
@@ -680,7 +708,7 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
       const int wave_row = 32 * wave;
       Rows<T, 2> rows;
       begin_rows<T, 2>(rows, [&](int r) { return query_of(first_row + wave_row + r); });
-      tall_item(rows, cache, kvh, table, item.from, item.to, scale, reinterpret_cast<char(*)[2 * TALL_BYTES]>(smem));
+      tall_item(rows, cache, kvh, table, item.from, item.to, scale, first_row + wave_row >= rows_all, reinterpret_cast<char(*)[2 * TALL_BYTES]>(smem));
       leave_rows<T, 2>(rows, rows_all - first_row - wave_row, o + (size_t)(item.at + wave_row) * D, lse + item.at + wave_row);
       return;
     } else {
