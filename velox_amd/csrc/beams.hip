@@ -504,8 +504,9 @@ extern "C" int velox_beam_most_vocab() { return MOST_VOCAB; }
 extern "C" long long velox_beam_scratch_bytes(int rows, int pieces, int keep) {
   return (long long)rows * pieces * ((long long)sizeof(PieceSum) + (long long)keep * (sizeof(uint64_t) + sizeof(Candidate)));
 }
+// outputs: [requests][keep] each of values (float32), beams and tokens (int32), one behind the other
 extern "C" int velox_beam_select(const float* logits, const float* scores, int requests, int beams, int vocab, int keep, int pieces, void* scratch,
-                                 long long scratch_bytes, float* out_scores, int* out_parents, int* out_tokens, hipStream_t stream) {
+                                 long long scratch_bytes, float* outputs, hipStream_t stream) {
   if (requests <= 0) return 0;
   const long long rows = (long long)requests * beams;
   if (beams < 1 || beams > MOST_BEAMS || vocab < 1 || vocab > MOST_VOCAB || keep < 1 || keep > MOST_KEPT || pieces < 1) return -1;
@@ -520,7 +521,8 @@ extern "C" int velox_beam_select(const float* logits, const float* scores, int r
   else beam_pieces_kernel<4><<<grid, THREADS, 0, stream>>>(logits, scores, vocab, span, keep, pieces, sums, candidates);
   const int status = (int)hipGetLastError();
   if (status != 0) return status;
-  beam_join_kernel<<<requests, JOIN_THREADS, 0, stream>>>(scores, sums, candidates, beams, keep, pieces, values, out_scores, out_parents, out_tokens);
+  beam_join_kernel<<<requests, JOIN_THREADS, 0, stream>>>(scores, sums, candidates, beams, keep, pieces, values, outputs, (int*)outputs + (size_t)requests * keep,
+                                                         (int*)outputs + 2 * (size_t)requests * keep);
   return (int)hipGetLastError();
 }
 

@@ -792,29 +792,6 @@ extern "C" int velox_shared_prefix_head_dim() { return D; }
 extern "C" int velox_shared_prefix_tall(int dtype) { return dtype == VELOX_BF16 && HAS_TALL ? TALL : 0; }
 extern "C" int velox_shared_prefix_most_row_tiles(int dtype) { return dtype == VELOX_BF16 ? most_row_tiles<bf16_t>() : most_row_tiles<float>(); }
 
-template <typename T>
-static int launch(const void* qkv, int qkv_stride, const void* k_cache, const void* v_cache, const int* block_tables, int table_width, const Lengths& l, int row_tiles,
-                  int items, const float* sinks, void* out, float* part_o, float* part_lse, Directory* directory, int nkv, int page_shift, int pages, float scale,
-                  hipStream_t stream) {
-  const Cache<T> cache{(const T*)k_cache, (const T*)v_cache, nkv, page_shift, (uint32_t)(pages - 1)};
-  constexpr int MOST = most_row_tiles<T>();
-  auto kernel = shared_prefix_kernel<T, 1>;
-  if constexpr (MOST >= 2) {
-    if (row_tiles == 2) kernel = shared_prefix_kernel<T, 2>;
-  }
-  if constexpr (MOST >= 4) {
-    if (row_tiles == 4) kernel = shared_prefix_kernel<T, 4>;
-  }
-  if constexpr (HAS_TALL && sizeof(T) == 2) {
-    if (row_tiles == TALL) kernel = shared_prefix_kernel<T, TALL>;
-  }
-  kernel<<<dim3(nkv, items), THREADS, 0, stream>>>((const T*)qkv, qkv_stride, cache, block_tables, table_width, l, scale, part_o, part_lse, directory);
-  const int status = (int)hipGetLastError();
-  if (status != 0) return status;
-  shared_prefix_join_kernel<T><<<dim3((nkv * l.group + JOIN_HEADS - 1) / JOIN_HEADS, l.num_seqs), 64 * JOIN_HEADS, 0, stream>>>(nkv * l.group, l.group, l.rows_room, directory, part_o, part_lse, sinks, (T*)out);
-  return (int)hipGetLastError();
-}
-
 // items: workgroups per KV head, and rows_room: rows per KV head, at least what velox_shared_prefix_room gives.  part_o: float32 [nkv, rows_room, D],
 // part_lse: float32 [nkv, rows_room], directory: eight int32 a sequence.  most_keys: no length counts beyond it.
 // An item has as many steps as the whole over `target`, the last of every row block fewer: at most `target` items and one for every row block, of which
@@ -824,22 +801,54 @@ extern "C" void velox_shared_prefix_room(int num_seqs, int num_groups, int group
   *items = target + blocks + own_blocks / WAVES + 2;
   *rows = target * (block_rows > 16 * WAVES ? block_rows : 16 * WAVES) + blocks * block_rows + own_blocks * 16 + 16 * WAVES;
 }
-extern "C" int velox_shared_prefix_attention(const void* qkv, int qkv_stride, const void* k_cache, const void* v_cache, const int* block_tables, int table_width,
-                                             const int* kv_lens, const int* group_starts, const int* shared_lens, int num_seqs, int num_groups, int nh, int nkv,
-                                             int page_shift, int pages, int most_keys, float scale, int row_tiles, int target, long long items, long long rows_room,
-                                             const float* sinks, void* out, float* part_o, float* part_lse, int* directory, int dtype, hipStream_t stream) {
-  if (num_seqs <= 0) return 0;
-  if (nkv < 1 || nh % nkv != 0 || page_shift < 3 || pages < 1 || most_keys < 0 || most_keys > (long long)table_width << page_shift || num_groups < 0 ||
-      num_groups > MOST_GROUPS || target < 1 || num_seqs > 65535 || items > 65535 || rows_room > 0x7fffffffLL) return -1;
-  if (row_tiles < 1 || (row_tiles & (row_tiles - 1)) != 0 || (row_tiles > velox_shared_prefix_most_row_tiles(dtype) && row_tiles != velox_shared_prefix_tall(dtype))) return -1;
-  const int group = nh / nkv;
+// What a call brings; the host packs it in this order (one argument costs it less than twenty-eight).
+struct SharedPrefixCall {
+  const void *qkv, *k_cache, *v_cache;
+  const int *block_tables, *kv_lens, *group_starts, *shared_lens;
+  const float* sinks;
+  void* out;
+  float *part_o, *part_lse;
+  int* directory;
+  long long rows_room;
+  int items, qkv_stride, table_width, num_seqs, num_groups, nh, nkv, page_shift, pages, most_keys, row_tiles, target, dtype;
+  float scale;
+};
+static_assert(sizeof(SharedPrefixCall) == 13 * 8 + 14 * 4, "as the host packs it");
+
+template <typename T>
+static int launch(const SharedPrefixCall& c, const Lengths& l, hipStream_t stream) {
+  const Cache<T> cache{(const T*)c.k_cache, (const T*)c.v_cache, c.nkv, c.page_shift, (uint32_t)(c.pages - 1)};
+  constexpr int MOST = most_row_tiles<T>();
+  Directory* const directory = (Directory*)c.directory;
+  auto kernel = shared_prefix_kernel<T, 1>;
+  if constexpr (MOST >= 2) {
+    if (c.row_tiles == 2) kernel = shared_prefix_kernel<T, 2>;
+  }
+  if constexpr (MOST >= 4) {
+    if (c.row_tiles == 4) kernel = shared_prefix_kernel<T, 4>;
+  }
+  if constexpr (HAS_TALL && sizeof(T) == 2) {
+    if (c.row_tiles == TALL) kernel = shared_prefix_kernel<T, TALL>;
+  }
+  kernel<<<dim3(c.nkv, c.items), THREADS, 0, stream>>>((const T*)c.qkv, c.qkv_stride, cache, c.block_tables, c.table_width, l, c.scale, c.part_o, c.part_lse, directory);
+  const int status = (int)hipGetLastError();
+  if (status != 0) return status;
+  shared_prefix_join_kernel<T><<<dim3((c.nh + JOIN_HEADS - 1) / JOIN_HEADS, l.num_seqs), 64 * JOIN_HEADS, 0, stream>>>(c.nh, l.group, l.rows_room, directory, c.part_o, c.part_lse,
+                                                                                                                c.sinks, (T*)c.out);
+  return (int)hipGetLastError();
+}
+
+extern "C" int velox_shared_prefix_attention(const SharedPrefixCall* call, hipStream_t stream) {
+  const SharedPrefixCall& c = *call;
+  if (c.num_seqs <= 0) return 0;
+  if (c.nkv < 1 || c.nh < 1 || c.nh % c.nkv != 0 || c.page_shift < 3 || c.pages < 1 || c.most_keys < 0 || c.most_keys > (long long)c.table_width << c.page_shift ||
+      c.num_groups < 0 || c.num_groups > MOST_GROUPS || c.target < 1 || c.num_seqs > 65535 || c.items > 65535 || c.rows_room > 0x7fffffffLL) return -1;
+  if (c.row_tiles < 1 || (c.row_tiles & (c.row_tiles - 1)) != 0 ||
+      (c.row_tiles > velox_shared_prefix_most_row_tiles(c.dtype) && c.row_tiles != velox_shared_prefix_tall(c.dtype))) return -1;
+  const int group = c.nh / c.nkv;
   long long least_items, least_rows;
-  velox_shared_prefix_room(num_seqs, num_groups, group, row_tiles, target, &least_items, &least_rows);
-  if (items < least_items || rows_room < least_rows) return -1;
-  const Lengths l{kv_lens, group_starts, shared_lens, num_seqs, num_groups, group, 16 * row_tiles, target, most_keys, (int)rows_room};
-  if (dtype == VELOX_BF16)
-    return launch<bf16_t>(qkv, qkv_stride, k_cache, v_cache, block_tables, table_width, l, row_tiles, (int)items, sinks, out, part_o, part_lse, (Directory*)directory, nkv,
-                          page_shift, pages, scale, stream);
-  return launch<float>(qkv, qkv_stride, k_cache, v_cache, block_tables, table_width, l, row_tiles, (int)items, sinks, out, part_o, part_lse, (Directory*)directory, nkv,
-                       page_shift, pages, scale, stream);
+  velox_shared_prefix_room(c.num_seqs, c.num_groups, group, c.row_tiles, c.target, &least_items, &least_rows);
+  if (c.items < least_items || c.rows_room < least_rows) return -1;
+  const Lengths l{c.kv_lens, c.group_starts, c.shared_lens, c.num_seqs, c.num_groups, group, 16 * c.row_tiles, c.target, c.most_keys, (int)c.rows_room};
+  return c.dtype == VELOX_BF16 ? launch<bf16_t>(c, l, stream) : launch<float>(c, l, stream);
 }

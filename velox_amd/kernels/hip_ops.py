@@ -18,6 +18,7 @@ import ctypes
 import functools
 import logging
 import os
+import struct
 import tempfile
 import threading
 from typing import Tuple, Dict, Optional, Sequence
@@ -41,6 +42,9 @@ class _StreamTerms(ctypes.Structure):
 
     _fields_ = [("term0", _P), ("term1", _P), ("mix", _P), ("out_w", _P), ("scale0", ctypes.c_float), ("scale1", ctypes.c_float),
                 ("term0_bf16", ctypes.c_int), ("term1_bf16", ctypes.c_int), ("num_terms", ctypes.c_int), ("unused", ctypes.c_int)]
+
+
+_SHARED_PREFIX_CALL = struct.Struct("=13q13if")  # ``SharedPrefixCall`` in shared_prefix.hip
 
 
 class KernelError(RuntimeError):
@@ -279,8 +283,7 @@ class HipOps:
         lib = self._shared_prefix.get(head_dim)
         if lib is None:
             lib = ctypes.CDLL(build.ensure_shared_prefix(head_dim))
-            lib.velox_shared_prefix_attention.argtypes = [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, ctypes.c_longlong, ctypes.c_longlong, _P, _P,
-                                                          _P, _P, _P, _I, _P]
+            lib.velox_shared_prefix_attention.argtypes = [ctypes.c_char_p, _P]
             lib.velox_shared_prefix_most_row_tiles.argtypes = [_I]
             for fn in (lib.velox_shared_prefix_attention, lib.velox_shared_prefix_most_row_tiles, lib.velox_shared_prefix_head_dim):
                 fn.restype = _I
@@ -295,7 +298,7 @@ class HipOps:
             lib = ctypes.CDLL(build.ensure_beams())
             lib.velox_beam_scratch_bytes.argtypes = [_I, _I, _I]
             lib.velox_beam_scratch_bytes.restype = ctypes.c_longlong
-            lib.velox_beam_select.argtypes = [_P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _P, _P, _P]
+            lib.velox_beam_select.argtypes = [_P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _P]
             lib.velox_reorder_states.argtypes = [_P, _I, _P, _P, _I, _I, _I, _P]
             for fn in (lib.velox_beam_select, lib.velox_reorder_states):
                 fn.restype = _I
@@ -2403,9 +2406,11 @@ class HipOps:
         # partial outputs, their log-sums, and where each sequence's rows of them lie, eight numbers
         rows_all = rows * num_kv_heads
         parts = workspace.get("shared_prefix_parts", rows_all * (head_dim + 1) + 8 * num_seqs).data_ptr()
-        self._call("shared_prefix_attention", self.shared_prefix_library(head_dim).velox_shared_prefix_attention, qkv_at, width, keys_at, values_at, tables_at, table_width,
-                   lens_at, starts_at, shared_at, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages, int(max_kv_len), float(scale), row_tiles,
-                   target, items, rows, sinks_at, out.data_ptr(), parts, parts + 4 * rows_all * head_dim, parts + 4 * rows_all * (head_dim + 1), code)
+        call = _SHARED_PREFIX_CALL.pack(
+            qkv_at, keys_at, values_at, tables_at, lens_at, starts_at, shared_at, sinks_at, out.data_ptr(), parts, parts + 4 * rows_all * head_dim,
+            parts + 4 * rows_all * (head_dim + 1), rows, items, width, table_width, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages,
+            int(max_kv_len), row_tiles, target, code, scale)
+        self._call("shared_prefix_attention", self.shared_prefix_library(head_dim).velox_shared_prefix_attention, call)
         return out
 
     def _beam_pieces(self, rows: int, vocab: int) -> int:
@@ -2432,17 +2437,16 @@ class HipOps:
         if rows > 65535:
             raise KernelError(f"beam_select: {rows} rows exceed the launch grid")
         device = self.device
-        values = torch.empty((requests, keep), dtype=torch.float32, device=device)
-        parents = torch.empty((requests, keep), dtype=torch.int32, device=device)
-        tokens = torch.empty((requests, keep), dtype=torch.int32, device=device)
+        outputs = torch.empty((3, requests, keep), dtype=torch.int32, device=device)
+        values, parents, tokens = outputs.unbind(0)
+        values = values.view(torch.float32)
         if requests == 0:
             return values, parents, tokens
         lib = self.beam_library()
         pieces = self._beam_pieces(rows, vocab)
         size = lib.velox_beam_scratch_bytes(rows, pieces, keep)
         scratch = torch.empty(size, dtype=torch.uint8, device=device)
-        self._call("beam_select", lib.velox_beam_select, logits_at, scores_at, requests, beams, vocab, keep, pieces, scratch.data_ptr(), size, values.data_ptr(),
-                   parents.data_ptr(), tokens.data_ptr())
+        self._call("beam_select", lib.velox_beam_select, logits_at, scores_at, requests, beams, vocab, keep, pieces, scratch.data_ptr(), size, outputs.data_ptr())
         return values, parents, tokens
 
     def reorder_states(self, tensors: Sequence[torch.Tensor], slots: torch.Tensor, parents: torch.Tensor, axis: int = 0) -> None:
