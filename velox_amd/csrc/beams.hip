@@ -54,18 +54,6 @@ __device__ __forceinline__ float just_below(float v) {  // -inf: -inf
   return v == 0.f ? -1.401298464e-45f : v > -INFINITY ? from_ordered(ordered_bits(v) - 1) : v;
 }
 
-__device__ __forceinline__ double wave_sum_64(double v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, VELOX_WAVE);
-  return v;
-}
-
-struct PieceSum { double sum; float top; int unused; };  // sum of exp(logit - top); top: a number near the greatest logit
-struct Candidate { float logit; int token; };            // token < 0: none
-
-constexpr int WAVES = THREADS / 64;
-constexpr int WAVE_LEFT = 512;  // a wave's list
-
 // The operation over the lanes of a row of 16, on every one of them.
 template <typename Op> __device__ __forceinline__ float over_row(float v, Op op) {
 #define VELOX_WITH(CONTROL) v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xf, 0xf, true)))
@@ -81,6 +69,38 @@ template <typename Op> __device__ __forceinline__ float over_wave(float v, Op op
   auto at = [&](int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); };
   return op(op(at(0), at(16)), op(at(32), at(48)));
 }
+
+// The same for 64 bits (any type of eight bytes).
+template <typename V, typename Op> __device__ __forceinline__ V over_row_64(V v, Op op) {
+  typedef int halves_t __attribute__((ext_vector_type(2)));
+#define VELOX_WITH(CONTROL)                                                              \
+  {                                                                                      \
+    halves_t x = __builtin_bit_cast(halves_t, v);                                        \
+    x[0] = __builtin_amdgcn_update_dpp(0, x[0], CONTROL, 0xf, 0xf, true);                \
+    x[1] = __builtin_amdgcn_update_dpp(0, x[1], CONTROL, 0xf, 0xf, true);                \
+    v = op(v, __builtin_bit_cast(V, x));                                                 \
+  }
+  VELOX_WITH(0xB1)
+  VELOX_WITH(0x4E)
+  VELOX_WITH(0x141)
+  VELOX_WITH(0x140)
+#undef VELOX_WITH
+  return v;
+}
+template <typename V, typename Op> __device__ __forceinline__ V over_wave_64(V v, Op op) {
+  typedef int halves_t __attribute__((ext_vector_type(2)));
+  v = over_row_64(v, op);
+  const halves_t x = __builtin_bit_cast(halves_t, v);
+  auto at = [&](int lane) { return __builtin_bit_cast(V, halves_t{__builtin_amdgcn_readlane(x[0], lane), __builtin_amdgcn_readlane(x[1], lane)}); };
+  return op(op(at(0), at(16)), op(at(32), at(48)));
+}
+struct Sum64 { __device__ __forceinline__ double operator()(double a, double b) const { return a + b; } };
+
+struct PieceSum { double sum; float top; int unused; };  // sum of exp(logit - top); top: a number near the greatest logit
+struct Candidate { float logit; int token; };            // token < 0: none
+
+constexpr int WAVES = THREADS / 64;
+constexpr int WAVE_LEFT = 512;  // a wave's list
 
 // Grid (pieces, rows); a piece is `span` tokens, a multiple of four, the row's last one may have fewer.  sums: [row][piece]; candidates:
 // [row][piece][keep], best first.  A round is UNITS loads of four tokens by every thread, the next one's in flight while one is worked.
@@ -227,7 +247,7 @@ __global__ void __launch_bounds__(THREADS) beam_pieces_kernel(const float* __res
   }
 
   // The waves' sums, and of their lists what reaches the greatest of their bounds.
-  sum = wave_sum_64(sum);
+  sum = over_wave_64(sum, Sum64());
   mine = over_wave(mine, greatest);
   if (lane == 0) {
     wave_tops[wave] = mine;
@@ -327,9 +347,8 @@ constexpr int MOST_BEAMS = 256, MOST_VOCAB = 1 << 24;
 // more candidates reach is looked for from the best value down in steps that double, then by halving the interval that is left, as a
 // number whose order is the values' (64 bits), and should too many have the very same value, among those by what else decides.  What the
 // bound leaves is ranked.  (Bounds from the lists' first entries alone leave nearly everything where the beams' scores lie far apart.)
-constexpr int JOIN_THREADS = 1024;
-constexpr int JOIN_WAVES = JOIN_THREADS / 64;
-constexpr int JOIN_HELD = 4;   // candidates a thread keeps in registers; the others' values lie in memory
+// (Few candidates are four waves' work: a count is a barrier, and its time goes by the waves that meet there.)
+constexpr int JOIN_HELD = 8;   // candidates a thread keeps in registers; the others' values lie in memory
 constexpr int JOIN_LEFT = 2 * MOST_KEPT + 64;
 
 __device__ __forceinline__ uint64_t ordered_bits_64(double v) {
@@ -338,9 +357,11 @@ __device__ __forceinline__ uint64_t ordered_bits_64(double v) {
 }
 __device__ __forceinline__ double from_ordered_64(uint64_t o) { return __longlong_as_double((long long)((o >> 63) != 0 ? o ^ 0x8000000000000000ull : ~o)); }
 
+template <int JOIN_THREADS>
 __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const float* __restrict__ scores, const PieceSum* __restrict__ sums, const Candidate* __restrict__ candidates,
                                                                  int beams, int keep, int pieces, uint64_t* __restrict__ values, float* __restrict__ out_scores,
                                                                  int* __restrict__ out_parents, int* __restrict__ out_tokens) {
+  constexpr int JOIN_WAVES = JOIN_THREADS / 64;
   __shared__ Place left[JOIN_LEFT];
   __shared__ double offsets[MOST_BEAMS], tops[MOST_BEAMS];
   __shared__ float beam_scores[MOST_BEAMS];
@@ -359,23 +380,25 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const float* __
     const int at = tid + k * JOIN_THREADS;
     held[k] = at < total ? mine[at] : Candidate{-INFINITY, -1};
   }
-  // a beam's maximum, and minus the logarithm of its sum
-  for (int w = wave; w < beams; w += JOIN_WAVES) {
+  // a beam's maximum, and minus the logarithm of its sum: sixteen lanes to a beam
+  for (int w = tid >> 4; w < beams; w += JOIN_THREADS / 16) {
+    const int first = tid & 15;
     const PieceSum* s = sums + (row0 + w) * pieces;
-    const PieceSum own = lane < pieces ? s[lane] : PieceSum{0.0, -INFINITY, 0};
+    const PieceSum own = first < pieces ? s[first] : PieceSum{0.0, -INFINITY, 0};
+    const float score = scores[row0 + w];
     float top = own.top;
-    for (int p = 64 + lane; p < pieces; p += 64) top = fmaxf(top, s[p].top);
-    top = wave_max(top);
+    for (int p = 16 + first; p < pieces; p += 16) top = fmaxf(top, s[p].top);
+    top = over_row(top, [](float a, float b) { return fmaxf(a, b); });
     auto part = [&](const PieceSum& x) {
       return x.top > -INFINITY ? (x.top == top ? x.sum : top < INFINITY ? x.sum * exp2_near_zero(((double)fmaxf(x.top, top - FAR_BELOW) - (double)top) * LOG2_E) : 0.0) : 0.0;
     };
     double sum = part(own);
-    for (int p = 64 + lane; p < pieces; p += 64) sum += part(s[p]);
-    sum = wave_sum_64(sum);
-    if (lane == 0) {
+    for (int p = 16 + first; p < pieces; p += 16) sum += part(s[p]);
+    sum = over_row_64(sum, Sum64());
+    if (first == 0) {
       tops[w] = (double)top;
       offsets[w] = top > -INFINITY ? -log(sum) : 0.0;
-      beam_scores[w] = scores[row0 + w];
+      beam_scores[w] = score;
     }
   }
   if (tid == 0) num_left = 0;
@@ -398,11 +421,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const float* __
     rest[at] = k;  // (read again by this thread alone)
     best = k > best ? k : best;
   }
-#pragma unroll
-  for (int offset = 1; offset < 64; offset <<= 1) {
-    const uint64_t other = (uint64_t)__shfl_xor((unsigned long long)best, offset, VELOX_WAVE);
-    best = other > best ? other : best;
-  }
+  best = over_wave_64(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
   if (lane == 0) wave_best[wave] = best;
   __syncthreads();
 #pragma unroll
@@ -521,8 +540,10 @@ extern "C" int velox_beam_select(const float* logits, const float* scores, int r
   else beam_pieces_kernel<4><<<grid, THREADS, 0, stream>>>(logits, scores, vocab, span, keep, pieces, sums, candidates);
   const int status = (int)hipGetLastError();
   if (status != 0) return status;
-  beam_join_kernel<<<requests, JOIN_THREADS, 0, stream>>>(scores, sums, candidates, beams, keep, pieces, values, outputs, (int*)outputs + (size_t)requests * keep,
-                                                         (int*)outputs + 2 * (size_t)requests * keep);
+  auto join = (long long)beams * pieces * keep <= 256 * JOIN_HELD ? beam_join_kernel<256> : beam_join_kernel<1024>;
+  join<<<requests, (long long)beams * pieces * keep <= 256 * JOIN_HELD ? 256 : 1024, 0, stream>>>(scores, sums, candidates, beams, keep, pieces, values, outputs,
+                                                                                              (int*)outputs + (size_t)requests * keep,
+                                                                                              (int*)outputs + 2 * (size_t)requests * keep);
   return (int)hipGetLastError();
 }
 
