@@ -202,6 +202,18 @@ def test_attention_result_does_not_hang_on_the_bounds(ops, workspace):
     b.check(b.run(ops, workspace, largest=4, longest=b.tables.shape[1] * 16))
 
 
+def test_attention_group_larger_than_said(ops, workspace):
+    """What a group has beyond ``largest_group`` reads all its keys through its own table."""
+    b = Batch(BF16, 12, 2, 128, 16, groups=[(4, 0), (5, 0)], lens=own(4, 450, 1, 50) + own(5, 90, 1, 50))
+    b.shared.copy_(torch.tensor([440, 80], dtype=torch.int32))
+    b.tables[1, :27] = b.tables[0, :27]  # (the first two of either share whole pages in earnest; the others have pages of their own)
+    b.tables[5, :5] = b.tables[4, :5]
+    b.k[b.tables[1, 27].long(), :, :8], b.v[b.tables[1, 27].long(), :, :, :8] = b.k[b.tables[0, 27].long(), :, :8], b.v[b.tables[0, 27].long(), :, :, :8]
+    got = b.run(ops, workspace, largest=2)
+    b.starts, b.shared = torch.tensor([0, 2, 4, 6], dtype=torch.int32).cuda(), torch.tensor([440, 0, 80], dtype=torch.int32).cuda()
+    b.check(got)
+
+
 def test_attention_agrees_with_paged_attention(ops, workspace):
     """Tables that are filled in full: the same answers as the kernels that read every sequence's keys."""
     g = torch.Generator().manual_seed(5)

@@ -73,7 +73,7 @@ template <> struct Block<float> {
 // ---- which workgroup does what -----------------------------------------------------------------------------------------
 // Everything is worked out from the lengths on the device, so that a captured step replays with other lengths.  A group's shared
 // keys are those of its first sequence at most (it is through that one's table that they are read); a sequence with fewer keys
-// than its group shares, and one that is alone in its group or in none, shares nothing.  A step is a tile of keys for each of four waves; all
+// than its group shares, one that is alone in its group or in none, and what a group has beyond `largest` share nothing.  A step is a tile of keys for each of four waves; all
 // items' steps over `target` workgroups are what one item may have (`per`: of a sequence's own keys, tiles of one wave).  A group's rows are cut
 // into blocks of `block_rows`, a sequence's G rows into blocks of 16.
 //
@@ -86,6 +86,7 @@ struct Lengths {
   const int* shared_lens;
   int num_seqs, num_groups, group, block_rows, target;  // group: query heads of a KV head
   int most;                                             // keys a table has room for
+  int largest;                                          // sequences of a group
   int rows_room;
 };
 
@@ -164,7 +165,8 @@ __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) 
   for (int b = lane; b < l.num_seqs && b < LENS_HELD; b += 64) plan.lens[b] = clamped(b < 64 ? len0 : l.kv_lens[b], 0, l.most);
   auto keys_of = [&](int b) { return b < LENS_HELD ? plan.lens[b] : clamped(l.kv_lens[b], 0, l.most); };
   for (int g = lane; g < l.num_groups; g += 64) {
-    const int start = clamped(g < 64 ? start0 : l.group_starts[g], 0, l.num_seqs), end = clamped(g < 64 ? end0 : l.group_starts[g + 1], start, l.num_seqs);
+    const int start = clamped(g < 64 ? start0 : l.group_starts[g], 0, l.num_seqs);
+    const int end = clamped(g < 64 ? end0 : l.group_starts[g + 1], start, min(l.num_seqs, start + l.largest));
     plan.start[g] = start;
     plan.end[g] = end;
     plan.shared[g] = end - start > 1 ? clamped(g < 64 ? shared0 : l.shared_lens[g], 0, keys_of(start)) : 0;
@@ -710,14 +712,13 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
       begin_rows<T, 2>(rows, [&](int r) { return query_of(first_row + wave_row + r); });
       tall_item(rows, cache, kvh, table, item.from, item.to, scale, first_row + wave_row >= rows_all, reinterpret_cast<char(*)[2 * TALL_BYTES]>(smem));
       leave_rows<T, 2>(rows, rows_all - first_row - wave_row, o + (size_t)(item.at + wave_row) * D, lse + item.at + wave_row);
-      return;
     } else {
-    Rows<T, RT> rows;
-    begin_rows<T, RT>(rows, [&](int r) { return query_of(first_row + r); });
-    stream_keys<T, RT>(rows, cache, kvh, table, item.from, item.to, item.from / TILE + wave, WAVES, scale);
-    join_waves<T, RT>(rows, rows_all - first_row, o + (size_t)item.at * D, lse + item.at, smem);
-    return;
+      Rows<T, RT> rows;
+      begin_rows<T, RT>(rows, [&](int r) { return query_of(first_row + r); });
+      stream_keys<T, RT>(rows, cache, kvh, table, item.from, item.to, item.from / TILE + wave, WAVES, scale);
+      join_waves<T, RT>(rows, rows_all - first_row, o + (size_t)item.at * D, lse + item.at, smem);
     }
+    return;
   }
   if (item.sequence < 0 || item.at + 16 > l.rows_room) return;
   if (item.tells && kvh == 0 && lane == 0) directory[item.sequence] = item.rows;
@@ -786,7 +787,7 @@ __global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int
 }
 
 // Row tiles a wave can hold: its registers hold the queries, the output and a tile of keys and values.
-template <typename T> constexpr int most_row_tiles() { return sizeof(T) * D <= 128 ? 4 : D <= 128 ? 2 : 1; }
+template <typename T> constexpr int most_row_tiles() { return D <= 128 ? 2 : 1; }
 
 extern "C" int velox_shared_prefix_head_dim() { return D; }
 extern "C" int velox_shared_prefix_tall(int dtype) { return dtype == VELOX_BF16 && HAS_TALL ? TALL : 0; }
@@ -795,9 +796,12 @@ extern "C" int velox_shared_prefix_most_row_tiles(int dtype) { return dtype == V
 // items: workgroups per KV head, and rows_room: rows per KV head, at least what velox_shared_prefix_room gives.  part_o: float32 [nkv, rows_room, D],
 // part_lse: float32 [nkv, rows_room], directory: eight int32 a sequence.  most_keys: no length counts beyond it.
 // An item has as many steps as the whole over `target`, the last of every row block fewer: at most `target` items and one for every row block, of which
-// the groups have num_seqs G / block_rows + num_groups at most and the sequences num_seqs ceil(G / 16), a quarter of a workgroup each.
-extern "C" void velox_shared_prefix_room(int num_seqs, int num_groups, int group, int row_tiles, int target, long long* items, long long* rows) {
-  const long long block_rows = 16LL * row_tiles, own_blocks = (long long)num_seqs * ((group + 15) / 16), blocks = (long long)num_seqs * group / block_rows + num_groups;
+// the groups have as many as all sequences' rows and one more each fill, or as many each as `largest` sequences do, and the sequences
+// ceil(G / 16) each, a quarter of a workgroup.
+extern "C" void velox_shared_prefix_room(int num_seqs, int num_groups, int group, int row_tiles, int target, int largest, long long* items, long long* rows) {
+  const long long block_rows = 16LL * row_tiles, own_blocks = (long long)num_seqs * ((group + 15) / 16);
+  const long long by_rows = (long long)num_seqs * group / block_rows + num_groups, by_groups = num_groups * (((long long)largest * group + block_rows - 1) / block_rows);
+  const long long blocks = by_rows < by_groups ? by_rows : by_groups;
   *items = target + blocks + own_blocks / WAVES + 2;
   *rows = target * (block_rows > 16 * WAVES ? block_rows : 16 * WAVES) + blocks * block_rows + own_blocks * 16 + 16 * WAVES;
 }
@@ -810,10 +814,11 @@ struct SharedPrefixCall {
   float *part_o, *part_lse;
   int* directory;
   long long rows_room;
-  int items, qkv_stride, table_width, num_seqs, num_groups, nh, nkv, page_shift, pages, most_keys, row_tiles, target, dtype;
+  int items, qkv_stride, table_width, num_seqs, num_groups, nh, nkv, page_shift, pages, most_keys, row_tiles, target, largest, dtype;
   float scale;
+  int unused;
 };
-static_assert(sizeof(SharedPrefixCall) == 13 * 8 + 14 * 4, "as the host packs it");
+static_assert(sizeof(SharedPrefixCall) == 13 * 8 + 16 * 4, "as the host packs it");
 
 template <typename T>
 static int launch(const SharedPrefixCall& c, const Lengths& l, hipStream_t stream) {
@@ -823,9 +828,6 @@ static int launch(const SharedPrefixCall& c, const Lengths& l, hipStream_t strea
   auto kernel = shared_prefix_kernel<T, 1>;
   if constexpr (MOST >= 2) {
     if (c.row_tiles == 2) kernel = shared_prefix_kernel<T, 2>;
-  }
-  if constexpr (MOST >= 4) {
-    if (c.row_tiles == 4) kernel = shared_prefix_kernel<T, 4>;
   }
   if constexpr (HAS_TALL && sizeof(T) == 2) {
     if (c.row_tiles == TALL) kernel = shared_prefix_kernel<T, TALL>;
@@ -842,13 +844,13 @@ extern "C" int velox_shared_prefix_attention(const SharedPrefixCall* call, hipSt
   const SharedPrefixCall& c = *call;
   if (c.num_seqs <= 0) return 0;
   if (c.nkv < 1 || c.nh < 1 || c.nh % c.nkv != 0 || c.page_shift < 3 || c.pages < 1 || c.most_keys < 0 || c.most_keys > (long long)c.table_width << c.page_shift ||
-      c.num_groups < 0 || c.num_groups > MOST_GROUPS || c.target < 1 || c.num_seqs > 65535 || c.items > 65535 || c.rows_room > 0x7fffffffLL) return -1;
+      c.num_groups < 0 || c.num_groups > MOST_GROUPS || c.target < 1 || c.largest < 1 || c.largest > c.num_seqs || c.num_seqs > 65535 || c.items > 65535 || c.rows_room > 0x7fffffffLL) return -1;
   if (c.row_tiles < 1 || (c.row_tiles & (c.row_tiles - 1)) != 0 ||
       (c.row_tiles > velox_shared_prefix_most_row_tiles(c.dtype) && c.row_tiles != velox_shared_prefix_tall(c.dtype))) return -1;
   const int group = c.nh / c.nkv;
   long long least_items, least_rows;
-  velox_shared_prefix_room(c.num_seqs, c.num_groups, group, c.row_tiles, c.target, &least_items, &least_rows);
+  velox_shared_prefix_room(c.num_seqs, c.num_groups, group, c.row_tiles, c.target, c.largest, &least_items, &least_rows);
   if (c.items < least_items || c.rows_room < least_rows) return -1;
-  const Lengths l{c.kv_lens, c.group_starts, c.shared_lens, c.num_seqs, c.num_groups, group, 16 * c.row_tiles, c.target, c.most_keys, (int)c.rows_room};
+  const Lengths l{c.kv_lens, c.group_starts, c.shared_lens, c.num_seqs, c.num_groups, group, 16 * c.row_tiles, c.target, c.most_keys, c.largest, (int)c.rows_room};
   return c.dtype == VELOX_BF16 ? launch<bf16_t>(c, l, stream) : launch<float>(c, l, stream);
 }

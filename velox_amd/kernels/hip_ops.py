@@ -44,7 +44,7 @@ class _StreamTerms(ctypes.Structure):
                 ("term0_bf16", ctypes.c_int), ("term1_bf16", ctypes.c_int), ("num_terms", ctypes.c_int), ("unused", ctypes.c_int)]
 
 
-_SHARED_PREFIX_CALL = struct.Struct("=13q13if")  # ``SharedPrefixCall`` in shared_prefix.hip
+_SHARED_PREFIX_CALL = struct.Struct("=13q14ifi")  # ``SharedPrefixCall`` in shared_prefix.hip
 
 
 class KernelError(RuntimeError):
@@ -2323,30 +2323,36 @@ class HipOps:
 
     @staticmethod
     @functools.lru_cache(maxsize=4096)
-    def _shared_prefix_shape(num_cus: int, num_seqs: int, num_groups: int, num_heads: int, num_kv_heads: int, head_dim: int, element_size: int, largest_group: int) -> Tuple[int, int, int, int]:
+    def _shared_prefix_shape(num_cus: int, num_seqs: int, num_groups: int, num_heads: int, num_kv_heads: int, head_dim: int, element_size: int, largest_group: int,
+                             max_kv_len: int) -> Tuple[int, int, int, int]:
         """Row tiles of a workgroup, over how many workgroups per KV head the keys are cut, and how many workgroups and rows of partial results
-        per KV head that makes at most (as ``velox_shared_prefix_room`` counts them)."""
+        per KV head that makes at most (as ``velox_shared_prefix_room`` counts them).
+
+        Row tiles go by the rows of the largest group: one or two of 16, or eight with tiles of keys in LDS (8).  Measured on MI355X (us, both kernels; 28 heads
+        over 4, one group): two / eight with 84 rows behind 8,192 keys 17.2 / 31.5, 224 22.7 / 23.9 and behind 32,768 52 / 49, 336 behind 8,192 33.7 / 28.1, behind 32,768
+        102 / 57, 448 behind 1,024 15.6 / 21.0, 4,096 25.2 / 24.8, 32,768 111 / 65; 320 of 64 channels behind 2,048 16.9 / 18.8, 16,384 44.8 / 37.8.  In float32 matrix
+        instructions decide and padded rows cost: one / two row tiles with 48 rows 16.7 / 19.7, 112 37.8 / 40.9, 28 32.3 / 31.2.
+        A workgroup per compute unit but where rows are many or float32 ones are in single tiles, two: one / two with 8 groups of 4 behind 1,024 to 2,048 keys 16.0 / 25.2
+        (more parts to join), 140 rows behind 8,192 19.7 / 22.0; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
         group = num_heads // num_kv_heads
-        most = 4 if element_size * head_dim <= 128 else 2 if head_dim <= 128 else 1
-        row_tiles = 1
-        while row_tiles < most and 16 * row_tiles < largest_group * group:
-            row_tiles *= 2
-        if element_size == 2 and head_dim in (64, 128) and largest_group * group > 64:
-            row_tiles = 8
-        # A workgroup per compute unit, two of the kernel for many rows.  Measured on MI355X (us, one / two): 8 groups of 4 behind 1,024 to 2,048 keys, 28 heads over 4,
-        # 12.6 + 4.2 and 13.8 + 12.2 (of which the second joins the parts), 5 of 8 in float32 15.8 and 21.4; 64 behind 8,192 keys 35.5 and 27.1, behind 32,768 161 and 109.
-        target = max(1, (2 if row_tiles == 8 else 1) * num_cus // num_kv_heads)
-        own_blocks, blocks = num_seqs * (-(-group // 16)), num_seqs * group // (16 * row_tiles) + num_groups
-        return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(16 * row_tiles, 64) + blocks * 16 * row_tiles + own_blocks * 16 + 64
+        rows = largest_group * group
+        row_tiles, per_unit = 1 if rows <= 16 or head_dim > 128 else 2, 1
+        if element_size == 2 and head_dim in (64, 128) and rows > 256 and max_kv_len >= 4096:
+            row_tiles, per_unit = 8, 2
+        elif element_size == 4 and row_tiles == 2 and -(-rows // 16) % 2 == 1:
+            row_tiles, per_unit = 1, 2
+        target = max(1, per_unit * num_cus // num_kv_heads)
+        block_rows, own_blocks = 16 * row_tiles, num_seqs * (-(-group // 16))
+        blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-rows // block_rows))
+        return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
 
     def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> int:
         """The most float32 elements ``shared_prefix_attention`` asks its workspace for (``shared_prefix_parts``) in any step of at most so many
         sequences and groups, whatever the lengths and the element type."""
-        rows = 0
-        for element_size in (2, 4):
-            for largest in (1, 1 << 20):
-                for groups in (0, max_num_groups):
-                    rows = max(rows, self._shared_prefix_shape(self.num_cus, max_num_seqs, groups, num_heads, num_kv_heads, head_dim, element_size, largest)[3])
+        group, rows = num_heads // num_kv_heads, 0
+        for row_tiles in (1, 2, 8):  # (whichever the largest group asks for)
+            blocks, own_blocks = max_num_seqs * group // (16 * row_tiles) + max_num_groups, max_num_seqs * (-(-group // 16))
+            rows = max(rows, max(1, 2 * self.num_cus // num_kv_heads) * max(16 * row_tiles, 64) + blocks * 16 * row_tiles + own_blocks * 16 + 64)
         return rows * num_kv_heads * (head_dim + 1) + 8 * max_num_seqs
 
     def shared_prefix_attention(self, qkv, num_heads, num_kv_heads, head_dim, k_cache, v_cache, block_size, block_tables, kv_lens, group_starts, shared_lens,
@@ -2359,7 +2365,7 @@ class HipOps:
         the block table of the group's FIRST sequence.  What a sequence has behind them is read through its own table, whose entries for
         pages that hold shared keys only are not looked at.  Sequences outside every group, alone in one, or with fewer keys than their group
         shares share nothing; a group shares no more keys than its first sequence has.  A sequence without keys gets zeros.
-        ``largest_group``: sequences of the largest group (which kernel is launched goes by it, the result does not), ``max_kv_len``: the most keys
+        ``largest_group``: at least the sequences of the largest group (what a group has beyond shares nothing either), ``max_kv_len``: the most keys
         of any sequence (a greater length counts as that many).  Lengths and groups are read on the device only: a captured call replays with other ones, as long as the number of
         sequences and groups stays.  ``sinks``: as for ``paged_attention``.  Pages hold at least 8 tokens."""
         num_seqs, num_groups = kv_lens.numel(), shared_lens.numel()
@@ -2400,7 +2406,8 @@ class HipOps:
         out = torch.empty((num_seqs, num_heads * head_dim), dtype=dtype, device=self.device)
         if num_seqs == 0:
             return out
-        row_tiles, target, items, rows = self._shared_prefix_shape(self.num_cus, num_seqs, num_groups, num_heads, num_kv_heads, head_dim, element_size, int(largest_group))
+        row_tiles, target, items, rows = self._shared_prefix_shape(self.num_cus, num_seqs, num_groups, num_heads, num_kv_heads, head_dim, element_size, int(largest_group),
+                                                                    int(max_kv_len))
         if items > 65535 or num_seqs > 65535:
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
         # partial outputs, their log-sums, and where each sequence's rows of them lie, eight numbers
@@ -2409,7 +2416,7 @@ class HipOps:
         call = _SHARED_PREFIX_CALL.pack(
             qkv_at, keys_at, values_at, tables_at, lens_at, starts_at, shared_at, sinks_at, out.data_ptr(), parts, parts + 4 * rows_all * head_dim,
             parts + 4 * rows_all * (head_dim + 1), rows, items, width, table_width, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages,
-            int(max_kv_len), row_tiles, target, code, scale)
+            int(max_kv_len), row_tiles, target, int(largest_group), code, scale, 0)
         self._call("shared_prefix_attention", self.shared_prefix_library(head_dim).velox_shared_prefix_attention, call)
         return out
 
