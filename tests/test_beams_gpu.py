@@ -398,6 +398,36 @@ def test_select_infinite_and_far_logits(ops):
     check_selection(ops, logits, scores, 5)
 
 
+@pytest.mark.parametrize("vocab", [3000, 40000])
+@pytest.mark.parametrize("about,spread", [(1e4, 400.0), (5e8, 100.0), (2.0 ** 30, 500.0), (2e9, 300.0), (1.7e10, 3000.0), (-1.7e10, 3000.0), (0.0, 1e30), (3e38, 3e36)])
+def test_select_logits_of_any_size(ops, vocab, about, spread):
+    """Where neighbouring numbers of 32 bits are further apart than exponentials reach, too."""
+    logits, scores = random_case(2, 3, vocab, seed=9, spread=spread)
+    check_selection(ops, logits + about, scores, 7)
+
+
+def test_select_rising_logits(ops):
+    """What a row's sum refers to moves again and again."""
+    logits = torch.linspace(-1.0, 1.0, 30000)[None] * torch.tensor([10.0, 2e3, 1e5, 1e9, 1e12, 3e38])[:, None]
+    check_selection(ops, logits, torch.zeros((3, 2)), 9)
+    check_selection(ops, logits.flip(1).contiguous(), torch.zeros((2, 3)), 9)
+
+
+def test_select_infinite_scores(ops):
+    """Every continuation is named once, also where infinity less infinity would be its worth."""
+    logits, scores = random_case(2, 3, 3000)
+    scores[:, 1] = math.inf
+    logits[1, 9] = math.inf
+    values, parents, tokens = (t.cpu() for t in ops.beam_select(logits.cuda(), scores.cuda(), 12))
+    assert values[0, 0] == math.inf and (parents[0, 0], tokens[0, 0]) == (1, 9) and (values[1] == math.inf).all() and (parents[1] == 1).all()
+    for r in range(2):
+        assert len(set(zip(parents[r].tolist(), tokens[r].tolist()))) == 12
+    best = torch.sort(logits[4], descending=True, stable=True).indices[:12]
+    assert tokens[1].tolist() == best.tolist()
+    rest = torch.sort((torch.log_softmax(logits.double(), 1)[:3] + scores[0].double()[:, None])[[0, 2]].view(-1), descending=True).values[:11]
+    assert ((values[0, 1:].double() - rest).abs() <= 2.0 ** -24 * rest.abs() + 1e-9).all()
+
+
 def test_select_rows_anywhere(ops):
     """Rows that begin at any multiple of four bytes."""
     logits, scores = random_case(2, 3, 10007)

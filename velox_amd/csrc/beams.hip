@@ -22,10 +22,11 @@
 constexpr int THREADS = 256;
 constexpr int MOST_KEPT = 64;
 
-// 2^t for -1000 <= t <= 1000 in 64 bits, to 6e-11 of it: t = k + f with |f| <= 1/2, and the polynomial of degree 7 that takes 2^f's values at the
-// Chebyshev points of that range.  (Adding 1.5 2^52 leaves k in the sum's low bits; it goes into the exponent.)
-__device__ __forceinline__ double exp2_near_zero(double t) {
-  const double shifted = t + 6755399441055744.0, f = t - (shifted - 6755399441055744.0);
+// e^x for -693 <= x <= 693 in 64 bits, to 6e-11 of it: x log2(e) = k + f with |f| <= 1/2, and the polynomial of degree 7 that takes 2^f's values at
+// the Chebyshev points of that range.  (Adding 1.5 2^52 leaves k in the sum's low bits; it goes into the exponent.)
+__device__ __forceinline__ double exp_in_range(double x) {
+  constexpr double LOG2_E = 1.4426950408889634074, ROUNDS = 6755399441055744.0;
+  const double shifted = fma(x, LOG2_E, ROUNDS), f = fma(x, LOG2_E, -(shifted - ROUNDS));
   double e = 1.5303699001378845e-05;
   e = fma(e, f, 0.00015469729140704658);
   e = fma(e, f, 0.0013333478480888061);
@@ -41,8 +42,16 @@ __device__ __forceinline__ double exp2_near_zero(double t) {
 }
 // the greater of the two, `a` if b is no number (one instruction; fmaxf takes another to quiet its operands)
 __device__ __forceinline__ float greater(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
-constexpr double LOG2_E = 1.4426950408889634074;
-constexpr float FAR_BELOW = 690.f;  // from here on a term is nothing beside 1
+// What is far below counts as nothing beside 1.  A wave's terms may exceed what they are relative to by e^ABOVE before that is moved; a term further
+// below it than BELOW counts as one that far; sums further apart than APART are not added.  (All within what exp_in_range takes, with what
+// 32 bits' rounding of the bounds adds below COARSE.  From there on numbers are 64 and more apart, and only the greatest themselves count.)
+constexpr float ABOVE = 600.f, BELOW = 640.f, COARSE = 1073741824.f;
+constexpr double APART = 690.0;
+// a sum of exponentials relative to `from`, relative to `to` >= from
+__device__ __forceinline__ double moved_sum(double sum, float from, float to) {
+  const double down = (double)to - (double)from;
+  return from == to ? sum : down < APART ? sum * exp_in_range(-down) : 0.0;
+}
 
 __device__ __forceinline__ uint32_t ordered_bits(float v) {  // compares like the number
   const uint32_t b = __float_as_uint(v);
@@ -213,22 +222,22 @@ __global__ void __launch_bounds__(THREADS) beam_pieces_kernel(const float* __res
       for (int e = 0; e < 4; ++e) take(!(v[e] > -INFINITY) && 4 * tid + e < min(keep, here), -INFINITY, 4 * tid + e);
     }
     bound = next_bound;
-    if (__ballot(most > ref + 600.f) != 0) {  // the first numbers, or far beyond all before
+    if (__ballot(most - ref > (fabsf(ref) < COARSE ? ABOVE : 0.f)) != 0) {  // the first numbers, or far beyond all before
       const float now = over_wave(most, greatest);
-      sum = ref > -INFINITY && now < INFINITY && ref > now - FAR_BELOW ? sum * exp2_near_zero(((double)ref - (double)now) * LOG2_E) : 0.0;
+      sum = moved_sum(sum, ref, now);
       ref = now;
     }
-    if (ref == INFINITY) {
+    if (!(fabsf(ref) < COARSE)) {
 #pragma unroll
-      for (int e = 0; e < PER_ROUND; ++e) sum += v[e] == INFINITY ? 1.0 : 0.0;
-    } else if (ref > -INFINITY) {
-      const double shift = -(double)ref * LOG2_E;
-      const float floor = ref - FAR_BELOW;
+      for (int e = 0; e < PER_ROUND; ++e) sum += v[e] == ref && ref > -INFINITY ? 1.0 : 0.0;
+    } else {
+      const double from = (double)ref;
+      const float floor = ref - BELOW;
       double second = 0.0;
 #pragma unroll
       for (int e = 0; e < PER_ROUND; e += 2) {
-        sum += exp2_near_zero(fma((double)greater(floor, v[e]), LOG2_E, shift));
-        second += exp2_near_zero(fma((double)greater(floor, v[e + 1]), LOG2_E, shift));
+        sum += exp_in_range((double)greater(floor, v[e]) - from);
+        second += exp_in_range((double)greater(floor, v[e + 1]) - from);
       }
       sum += second;
     }
@@ -326,10 +335,7 @@ __global__ void __launch_bounds__(THREADS) beam_pieces_kernel(const float* __res
   if (tid == 0) {
     double all = 0.0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float own = wave_refs[w];
-      if (own > -INFINITY) all += own == top ? wave_sums[w] : top < INFINITY ? wave_sums[w] * exp2_near_zero(((double)fmaxf(own, top - FAR_BELOW) - (double)top) * LOG2_E) : 0.0;
-    }
+    for (int w = 0; w < WAVES; ++w) all += moved_sum(wave_sums[w], wave_refs[w], top);
     sums[(size_t)row * pieces + piece] = PieceSum{all, top, 0};
   }
 }
@@ -389,9 +395,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const float* __
     float top = own.top;
     for (int p = 16 + first; p < pieces; p += 16) top = fmaxf(top, s[p].top);
     top = over_row(top, [](float a, float b) { return fmaxf(a, b); });
-    auto part = [&](const PieceSum& x) {
-      return x.top > -INFINITY ? (x.top == top ? x.sum : top < INFINITY ? x.sum * exp2_near_zero(((double)fmaxf(x.top, top - FAR_BELOW) - (double)top) * LOG2_E) : 0.0) : 0.0;
-    };
+    auto part = [&](const PieceSum& x) { return moved_sum(x.sum, x.top, top); };
     double sum = part(own);
     for (int p = 16 + first; p < pieces; p += 16) sum += part(s[p]);
     sum = over_row_64(sum, Sum64());
@@ -408,7 +412,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const float* __
     if (c.token < 0) return 0;
     const int w = beam_of(at);
     const double score = (double)beam_scores[w], top = tops[w];
-    return ordered_bits_64(!(c.logit > -INFINITY) || !(score > -INFINITY) ? -INFINITY : score + (((double)c.logit == top ? 0.0 : (double)c.logit - top) + offsets[w]));
+    const double value = score + (((double)c.logit == top ? 0.0 : (double)c.logit - top) + offsets[w]);
+    return ordered_bits_64(c.logit > -INFINITY && score > -INFINITY && value >= -INFINITY ? value : -INFINITY);  // (an infinite score less infinity is none)
   };
   uint64_t key[JOIN_HELD], best = 0;
 #pragma unroll
