@@ -65,6 +65,9 @@ def attention(**changed):
     (dict(largest_group=4), "largest group"),
     (dict(scale=0.0), "scale"),
     (dict(scale=math.nan), "scale"),
+    (dict(scale=1e39), "scale"),
+    (dict(block_size=131072), "block_size"),
+    (dict(block_size=65536, block_tables=torch.zeros((3, 513), dtype=torch.int32), max_kv_len=2 ** 25 + 1), "at most 33554432"),
     (dict(sinks=torch.zeros(5)), "sinks"),
     (dict(sinks=torch.zeros(4, dtype=torch.bfloat16)), "sinks"),
     (dict(workspace=None), "workspace"),
@@ -72,6 +75,12 @@ def attention(**changed):
 def test_attention_refuses(ops, changed, says):
     with pytest.raises(KernelError, match=says):
         ops.shared_prefix_attention(**attention(**changed))
+
+
+@pytest.mark.parametrize("num_seqs,longest", [(65536, 100), (65535, 1 << 20), (1025, 1 << 25)])
+def test_attention_refuses_more_than_it_counts(ops, num_seqs, longest):
+    with pytest.raises(KernelError, match="more than one call takes"):
+        ops._shared_prefix_shape(256, num_seqs, 1, 28, 4, 128, 2, 2, longest)
 
 
 def test_attention_of_no_sequences(ops):

@@ -182,6 +182,24 @@ def test_attention_many_sequences_and_groups(ops, workspace, dtype):
     b.check(b.run(ops, workspace))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("page", [128, 1024, 65536])
+@pytest.mark.parametrize("count,shared", [(3, 300), (70, 4100)])
+def test_attention_large_pages(ops, workspace, dtype, page, count, shared):
+    b = Batch(dtype, 8, 2, 64, page, groups=[(count, shared)], lens=own(count, shared, 1, 40))
+    b.check(b.run(ops, workspace))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("longest", [0, 1, 31, 64, 127, 130])
+def test_attention_lengths_beyond_the_most(ops, workspace, dtype, longest):
+    """They count as the most that was said, a group's shared keys among them."""
+    b = Batch(dtype, 8, 2, 64, 16, groups=[(5, 128)], lens=own(5, 128, 1, 40) + [200, 3], behind=2)
+    got = b.run(ops, workspace, longest=longest)
+    b.lens = b.lens.clamp(max=longest)
+    b.check(got)
+
+
 def test_attention_without_groups(ops, workspace):
     b = Batch(BF16, 12, 2, 128, 16, groups=[], lens=[100, 1, 333], behind=3)
     b.check(b.run(ops, workspace))

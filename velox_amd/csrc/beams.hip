@@ -40,8 +40,6 @@ __device__ __forceinline__ double exp_in_range(double x) {
   bits[1] += __builtin_bit_cast(halves_t, shifted)[0] << 20;
   return __builtin_bit_cast(double, bits);
 }
-// the greater of the two, `a` if b is no number (one instruction; fmaxf takes another to quiet its operands)
-__device__ __forceinline__ float greater(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 // What is far below counts as nothing beside 1.  A wave's terms may exceed what they are relative to by e^ABOVE before that is moved; a term further
 // below it than BELOW counts as one that far; sums further apart than APART are not added.  (All within what exp_in_range takes, with what
 // 32 bits' rounding of the bounds adds below COARSE.  From there on numbers are 64 and more apart, and only the greatest themselves count.)
@@ -233,11 +231,11 @@ __global__ void __launch_bounds__(THREADS) beam_pieces_kernel(const float* __res
     } else {
       const double from = (double)ref;
       const float floor = ref - BELOW;
-      double second = 0.0;
+      double second = 0.0;  // (what is no number counts as far below)
 #pragma unroll
       for (int e = 0; e < PER_ROUND; e += 2) {
-        sum += exp_in_range((double)greater(floor, v[e]) - from);
-        second += exp_in_range((double)greater(floor, v[e + 1]) - from);
+        sum += exp_in_range((double)fmaxf(floor, v[e]) - from);
+        second += exp_in_range((double)fmaxf(floor, v[e + 1]) - from);
       }
       sum += second;
     }

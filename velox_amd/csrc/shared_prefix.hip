@@ -31,7 +31,7 @@ constexpr int D = VELOX_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head size must be a multiple of 16 between 16 and 256");
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES;
-constexpr int MOST_GROUPS = 1024;
+constexpr int MOST_GROUPS = 1024, MOST_KEYS = 1 << 25;  // of a call, of a sequence
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
@@ -205,7 +205,7 @@ __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) 
   for (int base = 64; base < l.num_seqs; base += 64) tiles += own_blocks * tiles_of(own_of(base, latest));
   steps = __builtin_amdgcn_readlane(sum_up_to_lane(steps), 63);
   tiles = __builtin_amdgcn_readlane(sum_up_to_lane(tiles), 63);
-  int per = max(1, (steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target);
+  int per = clamped((steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target, 1, MOST_KEYS / 16);  // (nobody has more)
   if (l.block_rows > 16 * WAVES) {
     // (many rows: `target` workgroups fill the compute units, and the first one more would be a whole round; rounding parts up can bring it about)
     for (int tries = 0; tries < 6; ++tries) {
@@ -524,7 +524,7 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
   const uint32_t key_bytes = (uint32_t)(key_in_load * D + 8 * ((lane % PIECES) ^ ((first_key & 3) | ((first_key >> 3) & 1) << 2))) * 2;
   const int value_eight = (lane & 7) ^ ((lane >> 3) & 7);  // which eight of the tile's keys
   const size_t page_elems = ((size_t)cache.nkv * D) << cache.page_shift;
-  const uint32_t value_elems = (uint32_t)(kvh * D + 8 * wave + (lane >> 3)) << cache.page_shift;
+  const size_t value_elems = (size_t)(kvh * D + 8 * wave + (lane >> 3)) << cache.page_shift;
   // lane e's page id, e < 8, is that of the tile's keys 8 e .. 8 e + 7, or of the last keys there are
   auto load_id = [&](int n0) { return min((uint32_t)table[min(n0 + 8 * (lane & 7), hi - 1) >> cache.page_shift], cache.last_page); };
   auto issue_keys = [&](int n0, uint32_t id, int buffer) {
@@ -843,7 +843,7 @@ static int launch(const SharedPrefixCall& c, const Lengths& l, hipStream_t strea
 extern "C" int velox_shared_prefix_attention(const SharedPrefixCall* call, hipStream_t stream) {
   const SharedPrefixCall& c = *call;
   if (c.num_seqs <= 0) return 0;
-  if (c.nkv < 1 || c.nh < 1 || c.nh % c.nkv != 0 || c.page_shift < 3 || c.pages < 1 || c.most_keys < 0 || c.most_keys > (long long)c.table_width << c.page_shift ||
+  if (c.nkv < 1 || c.nh < 1 || c.nh % c.nkv != 0 || c.page_shift < 3 || c.page_shift > 16 || c.pages < 1 || c.most_keys < 0 || c.most_keys > MOST_KEYS || c.most_keys > (long long)c.table_width << c.page_shift ||
       c.num_groups < 0 || c.num_groups > MOST_GROUPS || c.target < 1 || c.largest < 1 || c.largest > c.num_seqs || c.num_seqs > 65535 || c.items > 65535 || c.rows_room > 0x7fffffffLL) return -1;
   if (c.row_tiles < 1 || (c.row_tiles & (c.row_tiles - 1)) != 0 ||
       (c.row_tiles > velox_shared_prefix_most_row_tiles(c.dtype) && c.row_tiles != velox_shared_prefix_tall(c.dtype))) return -1;

@@ -2317,7 +2317,7 @@ class HipOps:
         return out
 
     # -- several continuations of one prompt ------------------------------------------------------
-    MAX_PREFIX_GROUPS = 1024  # of one call of ``shared_prefix_attention``
+    MAX_PREFIX_GROUPS, MAX_PREFIX_KEYS = 1024, 1 << 25  # of one call of ``shared_prefix_attention``, of a sequence in it
     MAX_BEAMS, MAX_KEPT, MAX_BEAM_VOCAB = 256, 64, 1 << 24  # of ``beam_select``
     MAX_MOVED = 64  # beams of a request that ``reorder_states`` moves
 
@@ -2344,6 +2344,8 @@ class HipOps:
         target = max(1, per_unit * num_cus // num_kv_heads)
         block_rows, own_blocks = 16 * row_tiles, num_seqs * (-(-group // 16))
         blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-rows // block_rows))
+        if (own_blocks + blocks) * (max_kv_len // 16 + 2) > 0x7FFFFFFF or num_seqs > 65535:  # (tiles of keys are counted in 32 bits)
+            raise KernelError(f"shared_prefix_attention: {num_seqs} sequences of up to {max_kv_len} keys are more than one call takes")
         return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
 
     def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> int:
@@ -2367,7 +2369,7 @@ class HipOps:
         shares share nothing; a group shares no more keys than its first sequence has.  A sequence without keys gets zeros.
         ``largest_group``: at least the sequences of the largest group (what a group has beyond shares nothing either), ``max_kv_len``: the most keys
         of any sequence (a greater length counts as that many).  Lengths and groups are read on the device only: a captured call replays with other ones, as long as the number of
-        sequences and groups stays.  ``sinks``: as for ``paged_attention``.  Pages hold at least 8 tokens."""
+        sequences and groups stays.  ``sinks``: as for ``paged_attention``.  Pages hold 8 to 65,536 tokens."""
         num_seqs, num_groups = kv_lens.numel(), shared_lens.numel()
         dtype = qkv.dtype
         element_size = 2 if dtype == torch.bfloat16 else 4
@@ -2387,17 +2389,19 @@ class HipOps:
         starts_at = self._take("group_starts", group_starts, torch.int32, (num_groups + 1,))
         table_width = block_tables.shape[1] if block_tables.dim() == 2 else 0
         tables_at = self._take("block_tables", block_tables, torch.int32, (num_seqs, table_width))
-        if block_size < 8 or block_size & (block_size - 1):
-            raise KernelError(f"shared_prefix_attention: block_size must be a power of two from 8 on, got {block_size}")
+        if not 8 <= block_size <= 65536 or block_size & (block_size - 1):
+            raise KernelError(f"shared_prefix_attention: block_size must be a power of two from 8 to 65,536, got {block_size}")
         if max_kv_len < 0 or table_width * block_size < max_kv_len:
             raise KernelError(f"block tables of width {table_width} cannot cover {max_kv_len} keys")
+        if max_kv_len > self.MAX_PREFIX_KEYS:
+            raise KernelError(f"shared_prefix_attention: sequences of {max_kv_len} keys, at most {self.MAX_PREFIX_KEYS} are taken")
         pages = k_cache.shape[0]
         if pages < 1:
             raise KernelError("shared_prefix_attention: a cache without pages")
         keys_at = self._take("k_cache", k_cache, dtype, (pages, num_kv_heads, block_size, head_dim), 16)
         values_at = self._take("v_cache", v_cache, dtype, (pages, num_kv_heads, head_dim, block_size), 16)
-        if not 0 < scale < float("inf"):
-            raise KernelError(f"shared_prefix_attention: the scale must be positive, got {scale}")
+        if not 0 < scale < 2e38:
+            raise KernelError(f"shared_prefix_attention: the scale must be a positive number of 32 bits, got {scale}")
         sinks_at = 0 if sinks is None else self._take("sinks", sinks, torch.float32, (num_heads,))
         if not 1 <= largest_group <= max(num_seqs, 1):
             raise KernelError(f"shared_prefix_attention: a largest group of {largest_group} among {num_seqs} sequences")
@@ -2408,7 +2412,7 @@ class HipOps:
             return out
         row_tiles, target, items, rows = self._shared_prefix_shape(self.num_cus, num_seqs, num_groups, num_heads, num_kv_heads, head_dim, element_size, int(largest_group),
                                                                     int(max_kv_len))
-        if items > 65535 or num_seqs > 65535:
+        if items > 65535:
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
         # partial outputs, their log-sums, and where each sequence's rows of them lie, eight numbers
         rows_all = rows * num_kv_heads
