@@ -145,9 +145,8 @@ __device__ __forceinline__ int sum_up_to_lane(int v) {
 
 // The item of workgroup `wg`, and in it of this wave.  Every wave works it out for itself: a lane has a group and a sequence of its own, 64 of
 // each at a time; all waves write the same to `plan`, each reads what it has written itself, and the one barrier is behind the zeros that are written first.
-template <int TILE>
+template <int TILE, int STEP>
 __device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) {
-  constexpr int STEP = WAVES * TILE;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int own_blocks = (l.group + 15) / 16, block_shift = 31 - __builtin_clz(l.block_rows);
   auto at_most = [](int v, int count) { return v < count ? v : count - 1; };
@@ -694,7 +693,7 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
   constexpr int TILE = Block<T>::KB, R = 16 * RT, ROOM = RT == TALL ? 4 * TALL_BYTES : join_bytes<RT>();
   __shared__ __attribute__((aligned(1024))) char smem[sizeof(Plan) > ROOM ? sizeof(Plan) : ROOM];
   const int kvh = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Item item = find_item<TILE>(l, blockIdx.y, *reinterpret_cast<Plan*>(smem));
+  const Item item = find_item<TILE, (RT == TALL ? TALL_TILE : WAVES * TILE)>(l, blockIdx.y, *reinterpret_cast<Plan*>(smem));
   const int heads = l.group;
   float* const o = part_o + (size_t)kvh * l.rows_room * D;
   float* const lse = part_lse + (size_t)kvh * l.rows_room;
