@@ -200,6 +200,35 @@ def test_attention_lengths_beyond_the_most(ops, workspace, dtype, longest):
     b.check(got)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("count,shared", [(3, 300), (12, 1000), (63, 4200)])
+def test_attention_planned_ahead(ops, workspace, dtype, count, shared):
+    """More than 64 sequences or groups are planned by a kernel of its own, to the same items: others without a key, or groups without a
+    sequence, change nothing for the rows that were there."""
+    few = Batch(dtype, 28, 4, 128, 16, groups=[(count, shared)], lens=own(count, shared, 1, 300))
+    want = few.run(ops, workspace)
+    few.check(want)
+    many = Batch(dtype, 28, 4, 128, 16, groups=[(count, shared)], lens=own(count, shared, 1, 300) + [0] * (65 - count), behind=65 - count)
+    many.qkv[:count], many.k, many.v, many.tables[:count] = few.qkv, few.k, few.v, few.tables
+    for _ in range(20):
+        got = many.run(ops, workspace)
+        assert torch.equal(got[:count], want) and not got[count:].any()
+    few.starts, few.shared = torch.cat([few.starts, few.starts[-1:].repeat(64)]), torch.cat([few.shared, few.shared.repeat(64)])
+    for _ in range(20):
+        assert torch.equal(few.run(ops, workspace), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("groups", [61, 63, 64, 65, 127, 128, 129])
+def test_attention_about_a_waves_lanes(ops, workspace, dtype, groups):
+    sizes = [(1 + g % 3, 10 + 37 * (g % 7)) for g in range(groups)]
+    lens = [length for g, (count, shared) in enumerate(sizes) for length in own(count, shared, g % 2, 30)]
+    b = Batch(dtype, 4, 2, 64, 16, groups=sizes, lens=lens)
+    b.check(b.run(ops, workspace))
+    b = Batch(dtype, 4, 2, 64, 16, groups=[(2, 40)], lens=own(2, 40, 1, 9) + [7 * (i % 9) for i in range(groups - 2)], behind=groups - 2)
+    b.check(b.run(ops, workspace))
+
+
 def test_attention_without_groups(ops, workspace):
     b = Batch(BF16, 12, 2, 128, 16, groups=[], lens=[100, 1, 333], behind=3)
     b.check(b.run(ops, workspace))

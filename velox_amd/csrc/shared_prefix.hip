@@ -80,46 +80,26 @@ template <> struct Block<float> {
 // What the items leave has rows of its own, per KV head: `block_rows` for every item of a group, in the order groups, parts of the keys, row blocks, then
 // 16 for every item of a sequence, in the order sequences, parts, blocks.  Row r of a group's or of a sequence's part p then lies at
 // start + p stride + r.
+struct Directory { int shared_at, shared_stride, shared_parts, own_at, own_parts, unused[3]; };  // of a sequence: where its rows lie
+struct Item {           // group >= 0: of that group's shared keys, by the whole workgroup; else sequence >= 0: of its own keys, by one wave; else none
+  int group, sequence;
+  int first, count;     // the group's first sequence, and how many it has
+  int block, from, to;  // row block, keys
+  int at;               // its rows' place
+};
 struct Lengths {
   const int* kv_lens;
   const int* group_starts;
   const int* shared_lens;
+  const Item* planned;                                  // every wave's item, if there are more groups or sequences than a wave has lanes; or nullptr
   int num_seqs, num_groups, group, block_rows, target;  // group: query heads of a KV head
   int most;                                             // keys a table has room for
   int largest;                                          // sequences of a group
   int rows_room;
 };
-
-constexpr int LENS_HELD = 1024;
-struct Plan {  // in LDS
-  int start[MOST_GROUPS], end[MOST_GROUPS], shared[MOST_GROUPS];
-  int before[MOST_GROUPS];  // items of the groups before
-  int lens[LENS_HELD];
-  int begins[LENS_HELD];    // 1 + the group that begins at a sequence, or 0
-};
-struct Directory { int shared_at, shared_stride, shared_parts, own_at, own_parts, unused[3]; };  // of a sequence: where its rows lie
-struct Item {           // group >= 0: of that group's shared keys, by the whole workgroup; else sequence >= 0: of its own keys, by this wave; else none
-  int group, sequence;
-  int first, count;     // the group's first sequence, and how many it has
-  int block, from, to;  // row block, keys
-  int at;               // its rows' place
-  bool tells;           // it writes the directory
-  Directory rows;
-};
+struct Own { int group, from, to; };  // a sequence's own keys [from, to); group: whose shared keys it has, or -1
 
 __device__ __forceinline__ int clamped(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
-// the greatest of v >= 0 and those of the lanes before
-__device__ __forceinline__ int most_up_to_lane(int v) {
-#define VELOX_MAX_SHIFTED(CONTROL, ROWS) v = max(v, __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false))
-  VELOX_MAX_SHIFTED(0x111, 0xf);
-  VELOX_MAX_SHIFTED(0x112, 0xf);
-  VELOX_MAX_SHIFTED(0x114, 0xf);
-  VELOX_MAX_SHIFTED(0x118, 0xf);
-  VELOX_MAX_SHIFTED(0x142, 0xa);
-  VELOX_MAX_SHIFTED(0x143, 0xc);
-#undef VELOX_MAX_SHIFTED
-  return v;
-}
 // a / b rounded down, 0 <= a < 2^23 <= 2^31 / b: by the reciprocal, which is off by one at most
 __device__ __forceinline__ int quotient(int a, int b) {
   int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
@@ -130,147 +110,223 @@ __device__ __forceinline__ int quotient(int a, int b) {
 }
 __device__ __forceinline__ int parts_of(int steps, int per) { return quotient(steps + per - 1, per); }
 
-// v plus those of the lanes before
+// the operation over v and those of the lanes before
+#define VELOX_UP_TO_LANE(OP)                                                                           \
+  OP(0x111, 0xf); /* from 1, 2, 4 and 8 lanes down in a row of 16, */                                  \
+  OP(0x112, 0xf);                                                                                      \
+  OP(0x114, 0xf);                                                                                      \
+  OP(0x118, 0xf);                                                                                      \
+  OP(0x142, 0xa); /* from the end of the row before, into the second and the fourth, */                \
+  OP(0x143, 0xc); /* from the middle, into the upper half */
 __device__ __forceinline__ int sum_up_to_lane(int v) {
 #define VELOX_ADD_SHIFTED(CONTROL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false)
-  VELOX_ADD_SHIFTED(0x111, 0xf);  // from 1, 2, 4 and 8 lanes down in a row of 16,
-  VELOX_ADD_SHIFTED(0x112, 0xf);
-  VELOX_ADD_SHIFTED(0x114, 0xf);
-  VELOX_ADD_SHIFTED(0x118, 0xf);
-  VELOX_ADD_SHIFTED(0x142, 0xa);  // from the end of the row before, into the second and the fourth,
-  VELOX_ADD_SHIFTED(0x143, 0xc);  // from the middle, into the upper half
+  VELOX_UP_TO_LANE(VELOX_ADD_SHIFTED)
 #undef VELOX_ADD_SHIFTED
   return v;
 }
+__device__ __forceinline__ int most_up_to_lane(int v) {  // v >= 0
+#define VELOX_MAX_SHIFTED(CONTROL, ROWS) v = max(v, __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false))
+  VELOX_UP_TO_LANE(VELOX_MAX_SHIFTED)
+#undef VELOX_MAX_SHIFTED
+  return v;
+}
+#undef VELOX_UP_TO_LANE
 
-// The item of workgroup `wg`, and in it of this wave.  Every wave works it out for itself: a lane has a group and a sequence of its own, 64 of
-// each at a time; all waves write the same to `plan`, each reads what it has written itself, and the one barrier is behind the zeros that are written first.
-template <int TILE, int STEP>
-__device__ __forceinline__ Item find_item(const Lengths& l, int wg, Plan& plan) {
+// Numbers of a plan, by the keys of a tile and of a group's step (powers of two).
+struct Counts {
+  int tile_shift, step_shift, block_shift, own_blocks;
+  __device__ __forceinline__ Counts(const Lengths& l, int tile_shift, int step_shift)
+      : tile_shift(tile_shift), step_shift(step_shift), block_shift(31 - __builtin_clz(l.block_rows)), own_blocks((l.group + 15) / 16) {}
+  __device__ __forceinline__ int steps(int keys) const { return (keys + (1 << step_shift) - 1) >> step_shift; }
+  __device__ __forceinline__ int tiles(const Own& own) const { return own.to > own.from ? ((own.to + (1 << tile_shift) - 1) >> tile_shift) - (own.from >> tile_shift) : 0; }
+  __device__ __forceinline__ int blocks(const Lengths& l, int count, int shared) const { return shared > 0 ? (count * l.group + l.block_rows - 1) >> block_shift : 0; }
+  __device__ __forceinline__ int per(const Lengths& l, int steps, int tiles) const {
+    return clamped((steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target, 1, MOST_KEYS / 16);  // (nobody has more)
+  }
+  // (many rows: `target` workgroups fill the compute units, and the first one more would be a whole round; rounding parts up can bring it about)
+  static constexpr int TRIES = 6;
+  __device__ __forceinline__ bool fills_units(const Lengths& l) const { return l.block_rows > 16 * WAVES; }
+  static __device__ __forceinline__ int raised(int per) { return per + 1 + (per >> 4); }
+  __device__ __forceinline__ Item of_group(const Lengths& l, int item, int place, int group, int first, int count, int shared, int per) const {
+    const int row_blocks = blocks(l, count, shared), part = quotient(place, row_blocks), from = (part * per) << step_shift;
+    return Item{group, -1, first, count, place - part * row_blocks, from, min(from + (per << step_shift), shared), item << block_shift};
+  }
+  __device__ __forceinline__ Item of_sequence(int item, int place, int sequence, int from, int to, int per, int group_items) const {
+    const int part = quotient(place, own_blocks), low = ((from >> tile_shift) + part * per) << tile_shift;
+    return Item{-1, sequence, 0, 0, place - part * own_blocks, max(low, from), min(low + (per << tile_shift), to), (group_items << block_shift) + item * 16};
+  }
+};
+__device__ __forceinline__ Own own_keys(int group, int shared, int len) { return shared > 0 && shared <= len ? Own{group, shared, len} : Own{-1, 0, len}; }
+
+// With up to 64 sequences and groups every wave works its item out for itself: a lane has a group and a sequence of its own.  (1.7 us; with 240
+// sequences, 64 at a time, it was 7 of 24.5 us, with 1,000 68 of 145.)  `begins`: this wave's 64 places in LDS.
+__device__ __forceinline__ Item find_item(const Lengths& l, const Counts& counts, int wg, int* begins, Directory* __restrict__ directory) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int own_blocks = (l.group + 15) / 16, block_shift = 31 - __builtin_clz(l.block_rows);
   auto at_most = [](int v, int count) { return v < count ? v : count - 1; };
-  // (everything that a lane's first group and sequence need is asked for before any of it is waited for)
-  int start0 = 0, end0 = 0, shared0 = 0;
+  int start = 0, end = 0, shared = 0;
   if (l.num_groups > 0) {
     const int g = at_most(lane, l.num_groups);
-    start0 = l.group_starts[g];
-    end0 = l.group_starts[g + 1];
-    shared0 = l.shared_lens[g];
+    start = l.group_starts[g];
+    end = l.group_starts[g + 1];
+    shared = l.shared_lens[g];
   }
-  const int len0 = l.kv_lens[at_most(lane, l.num_seqs)];
-  for (int b = threadIdx.x; b < l.num_seqs && b < LENS_HELD; b += THREADS) plan.begins[b] = 0;
+  int len = l.kv_lens[at_most(lane, l.num_seqs)];
+  begins[lane] = 0;
+  len = lane < l.num_seqs ? clamped(len, 0, l.most) : 0;
+  start = clamped(start, 0, l.num_seqs);
+  end = clamped(end, start, min(l.num_seqs, start + l.largest));
+  shared = clamped(shared, 0, __shfl(len, start & 63, VELOX_WAVE));
+  if (lane >= l.num_groups || end - start < 2) shared = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a wave's accesses to LDS are done in order)
+  if (lane < l.num_groups && end > start) begins[start] = lane + 1;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const int group = most_up_to_lane(begins[lane]) - 1;  // the last that begins at this lane's sequence or before, or -1
+  const int its_end = __shfl(end, group & 63, VELOX_WAVE), its_shared = __shfl(shared, group & 63, VELOX_WAVE);
+  const Own own = own_keys(group, group >= 0 && lane < its_end ? its_shared : 0, len);
+
+  const int blocks = counts.blocks(l, end - start, shared), steps = counts.steps(shared), tiles = counts.tiles(own);
+  auto sum = [](int v) { return __builtin_amdgcn_readlane(sum_up_to_lane(v), 63); };
+  int per = counts.per(l, sum(blocks * steps), sum(counts.own_blocks * tiles));
+  if (counts.fills_units(l)) {
+    for (int tries = 0; tries < Counts::TRIES && sum(blocks * parts_of(steps, per)) > l.target; ++tries) per = Counts::raised(per);
+  }
+  const int items = blocks * parts_of(steps, per), upto = sum_up_to_lane(items), group_items = __builtin_amdgcn_readlane(upto, 63);
+  auto of = [](int v, int at) { return __builtin_amdgcn_readlane(v, at); };
+  if (wg < group_items) {
+    const int at = __ffsll((unsigned long long)__ballot(upto > wg)) - 1, first = of(start, at);
+    return counts.of_group(l, wg, wg - of(upto - items, at), at, first, of(end, at) - first, of(shared, at), per);
+  }
+  // every sequence has one item at least; its first one's wave writes down where its rows lie
+  const int item = (wg - group_items) * WAVES + wave, parts = max(1, parts_of(tiles, per)), own_items = lane < l.num_seqs ? counts.own_blocks * parts : 0;
+  const int own_upto = sum_up_to_lane(own_items);
+  const uint64_t holds = __ballot(own_upto > item);
+  if (holds == 0) return Item{-1, -1, 0, 0, 0, 0, 0, 0};
+  const int at = __ffsll((unsigned long long)holds) - 1, first = of(own_upto - own_items, at), from = of(own.from, at), its_group = of(own.group, at);
+  if (item == first && blockIdx.x == 0) {
+    Directory rows = {0, 0, 0, (group_items << counts.block_shift) + first * 16, of(parts, at), {}};
+    if (its_group >= 0) {
+      rows.shared_at = (of(upto - items, its_group) << counts.block_shift) + (at - of(start, its_group)) * l.group;
+      rows.shared_stride = of(blocks, its_group) << counts.block_shift;
+      rows.shared_parts = parts_of(counts.steps(from), per);
+    }
+    if (lane == 0) directory[at] = rows;
+  }
+  return counts.of_sequence(item, item - first, at, from, of(own.to, at), per, group_items);
+}
+
+// With more of either a workgroup ahead works all items out: a thread has a group and a sequence of its own (of these as many at a time), then every item is
+// looked up by halving.  planned: [workgroup][wave], a group's item four times.
+constexpr int PLAN_THREADS = 1024;
+static_assert(MOST_GROUPS <= PLAN_THREADS, "a thread has a group");
+__global__ void __launch_bounds__(PLAN_THREADS) shared_prefix_plan_kernel(const Lengths l, int tile_shift, int step_shift, int workgroups, Item* __restrict__ planned,
+                                                                          Directory* __restrict__ directory) {
+  __shared__ int lens[PLAN_THREADS], start[MOST_GROUPS], end[MOST_GROUPS], shared[MOST_GROUPS], before[MOST_GROUPS];
+  __shared__ int upto[PLAN_THREADS], from[PLAN_THREADS], to[PLAN_THREADS];
+  typedef int two_t __attribute__((ext_vector_type(2)));
+  __shared__ two_t wave_sums[2][PLAN_THREADS / 64];
+  const Counts counts(l, tile_shift, step_shift);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = blockDim.x;  // (as many as there are groups, at least)
+  int turn = 0;
+  struct Sums { int groups, own, all_groups, all_own; };  // up to this thread, and of all
+  auto sums_up_to_thread = [&](int groups, int own) {
+    const two_t in_wave = {sum_up_to_lane(groups), sum_up_to_lane(own)};
+    turn ^= 1;
+    if (lane == 63) wave_sums[turn][wave] = in_wave;
+    __syncthreads();
+    const two_t other = lane < threads / 64 ? wave_sums[turn][lane] : two_t{0, 0};
+    const int others[2] = {sum_up_to_lane(other[0]), sum_up_to_lane(other[1])};
+    const int before_wave = __builtin_amdgcn_readfirstlane(wave) - 1;
+    Sums sums = {in_wave[0], in_wave[1], __builtin_amdgcn_readlane(others[0], 63), __builtin_amdgcn_readlane(others[1], 63)};
+    if (before_wave >= 0) {
+      sums.groups += __builtin_amdgcn_readlane(others[0], before_wave);
+      sums.own += __builtin_amdgcn_readlane(others[1], before_wave);
+    }
+    return sums;
+  };
+  auto keys_of = [&](int b) { return clamped(l.kv_lens[b], 0, l.most); };
+  int first = 0, behind = 0, keys = 0;
+  if (tid < l.num_groups) {
+    first = l.group_starts[tid];
+    behind = l.group_starts[tid + 1];
+    keys = l.shared_lens[tid];
+  }
+  const int len0 = tid < l.num_seqs ? keys_of(tid) : 0;
+  lens[tid] = len0;
   __syncthreads();
-  for (int b = lane; b < l.num_seqs && b < LENS_HELD; b += 64) plan.lens[b] = clamped(b < 64 ? len0 : l.kv_lens[b], 0, l.most);
-  auto keys_of = [&](int b) { return b < LENS_HELD ? plan.lens[b] : clamped(l.kv_lens[b], 0, l.most); };
-  for (int g = lane; g < l.num_groups; g += 64) {
-    const int start = clamped(g < 64 ? start0 : l.group_starts[g], 0, l.num_seqs);
-    const int end = clamped(g < 64 ? end0 : l.group_starts[g + 1], start, min(l.num_seqs, start + l.largest));
-    plan.start[g] = start;
-    plan.end[g] = end;
-    plan.shared[g] = end - start > 1 ? clamped(g < 64 ? shared0 : l.shared_lens[g], 0, keys_of(start)) : 0;
-    if (end > start && start < LENS_HELD) plan.begins[start] = g + 1;
+  int steps = 0, blocks = 0;
+  if (tid < l.num_groups) {
+    first = clamped(first, 0, l.num_seqs);
+    behind = clamped(behind, first, min(l.num_seqs, first + l.largest));
+    keys = behind - first > 1 ? clamped(keys, 0, first < threads ? lens[first] : keys_of(first)) : 0;
+    start[tid] = first;
+    end[tid] = behind;
+    shared[tid] = keys;
+    steps = counts.steps(keys);
+    blocks = counts.blocks(l, behind - first, keys);
   }
-  struct Own { int group, from, to; };  // a sequence's own keys [from, to); group: whose shared keys it has, or -1
-  // of sequence base + lane; `latest` is 1 + the last group that begins before `base`, or 0, and on return before base + 64
-  auto own_of = [&](int base, int& latest) {
-    const int b = base + lane;
-    int group = 0;
-    if (base + 64 <= LENS_HELD) {
-      group = max(most_up_to_lane(b < l.num_seqs ? plan.begins[b] : 0), latest);
-      latest = __builtin_amdgcn_readlane(group, 63);
-    } else {
-      int lo = -1, hi = l.num_groups;  // the last group that begins at b or before
+  __syncthreads();
+  auto own_of = [&](int b, int keys) {
+    int lo = -1, hi = l.num_groups;  // the last group that begins at b or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start[mid] <= b) lo = mid;
+      else hi = mid;
+    }
+    return own_keys(lo, lo >= 0 && b < end[lo] ? shared[lo] : 0, keys);
+  };
+  Own own = tid < l.num_seqs ? own_of(tid, len0) : Own{-1, 0, 0};
+  int tiles = counts.tiles(own);
+  for (int b = threads + tid; b < l.num_seqs; b += threads) tiles += counts.tiles(own_of(b, keys_of(b)));
+  const Sums work = sums_up_to_thread(blocks * steps, counts.own_blocks * tiles);
+  int per = counts.per(l, work.all_groups, work.all_own);
+  if (counts.fills_units(l)) {
+    for (int tries = 0; tries < Counts::TRIES && sums_up_to_thread(blocks * parts_of(steps, per), 0).all_groups > l.target; ++tries) per = Counts::raised(per);
+  }
+  const int items = blocks * parts_of(steps, per);
+  int group_items = 0, own_items = 0;
+  for (int base = 0; base < l.num_seqs; base += threads) {
+    const int b = base + tid;
+    if (base > 0) own = b < l.num_seqs ? own_of(b, keys_of(b)) : Own{-1, 0, 0};
+    const int parts = max(1, parts_of(counts.tiles(own), per)), its_items = b < l.num_seqs ? counts.own_blocks * parts : 0;
+    const Sums sums = sums_up_to_thread(items, its_items);  // (its barrier: everybody is done with what the sequences before have left here)
+    group_items = sums.all_groups;
+    if (base == 0 && tid < l.num_groups) before[tid] = sums.groups - items;
+    upto[tid] = sums.own;
+    from[tid] = own.from;
+    to[tid] = own.to;
+    __syncthreads();
+    if (b < l.num_seqs) {
+      Directory rows = {0, 0, 0, (group_items << counts.block_shift) + (own_items + sums.own - its_items) * 16, parts, {}};
+      if (own.group >= 0) {
+        rows.shared_at = (before[own.group] << counts.block_shift) + (b - start[own.group]) * l.group;
+        rows.shared_stride = counts.blocks(l, end[own.group] - start[own.group], shared[own.group]) << counts.block_shift;
+        rows.shared_parts = parts_of(counts.steps(own.from), per);
+      }
+      directory[b] = rows;
+    }
+    for (int t = tid; t < sums.all_own; t += threads) {
+      int lo = -1, hi = threads - 1;  // the first sequence that has an item behind t
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (plan.start[mid] <= b) lo = mid;
-        else hi = mid;
+        if (upto[mid] > t) hi = mid;
+        else lo = mid;
       }
-      group = lo + 1;
+      const int item = own_items + t, record = group_items * WAVES + item;
+      if (record < workgroups * WAVES) planned[record] = counts.of_sequence(item, t - (hi > 0 ? upto[hi - 1] : 0), base + hi, from[hi], to[hi], per, group_items);
     }
-    if (b >= l.num_seqs) return Own{-1, 0, 0};
-    const int len = keys_of(b), shared = group > 0 && b < plan.end[group - 1] ? plan.shared[group - 1] : 0;
-    return shared > 0 && shared <= len ? Own{group - 1, shared, len} : Own{-1, 0, len};
-  };
-  auto blocks_of = [&](int g) { return plan.shared[g] > 0 ? ((plan.end[g] - plan.start[g]) * l.group + l.block_rows - 1) >> block_shift : 0; };
-  auto steps_of = [&](int keys) { return (unsigned)(keys + STEP - 1) / STEP; };
-  auto tiles_of = [&](const Own& own) { return own.to > own.from ? (int)((unsigned)(own.to + TILE - 1) / TILE - (unsigned)own.from / TILE) : 0; };
-  // steps of all items, and how many one may have
-  int latest = 0;
-  const Own own0 = own_of(0, latest);
-  const int latest0 = latest;
-  int steps = 0, tiles = own_blocks * tiles_of(own0);
-  for (int g = lane; g < l.num_groups; g += 64) steps += blocks_of(g) * steps_of(plan.shared[g]);
-  for (int base = 64; base < l.num_seqs; base += 64) tiles += own_blocks * tiles_of(own_of(base, latest));
-  steps = __builtin_amdgcn_readlane(sum_up_to_lane(steps), 63);
-  tiles = __builtin_amdgcn_readlane(sum_up_to_lane(tiles), 63);
-  int per = clamped((steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target, 1, MOST_KEYS / 16);  // (nobody has more)
-  if (l.block_rows > 16 * WAVES) {
-    // (many rows: `target` workgroups fill the compute units, and the first one more would be a whole round; rounding parts up can bring it about)
-    for (int tries = 0; tries < 6; ++tries) {
-      int items = 0;
-      for (int g = lane; g < l.num_groups; g += 64) items += blocks_of(g) * parts_of(steps_of(plan.shared[g]), per);
-      if (__builtin_amdgcn_readlane(sum_up_to_lane(items), 63) <= l.target) break;
-      per += 1 + (per >> 4);
-    }
+    own_items += sums.all_own;
   }
-  // the groups' items
-  Item found = {-1, -1, 0, 0, 0, 0, 0, 0, false, {}};
-  int before = 0;
-  for (int base = 0; base < l.num_groups; base += 64) {
-    const int g = base + lane;
-    const int blocks = g < l.num_groups ? blocks_of(g) : 0, items = blocks > 0 ? blocks * parts_of(steps_of(plan.shared[g]), per) : 0;
-    const int upto = before + sum_up_to_lane(items);
-    if (g < l.num_groups) plan.before[g] = upto - items;
-    const uint64_t holds = __ballot(upto > wg);
-    if (holds != 0) {
-      const int at = __ffsll((unsigned long long)holds) - 1;
-      const int place = wg - __builtin_amdgcn_readlane(upto - items, at), row_blocks = __builtin_amdgcn_readlane(blocks, at), part = quotient(place, row_blocks);
-      found.group = base + at;
-      found.first = __builtin_amdgcn_readfirstlane(plan.start[base + at]);
-      found.count = __builtin_amdgcn_readfirstlane(plan.end[base + at]) - found.first;
-      found.block = place - part * row_blocks;
-      found.from = part * per * STEP;
-      found.to = min(found.from + per * STEP, __builtin_amdgcn_readfirstlane(plan.shared[base + at]));
-      found.at = wg << block_shift;
-      return found;
+  for (int record = tid; record < group_items * WAVES && record < workgroups * WAVES; record += threads) {
+    const int item = record / WAVES;
+    int lo = 0, hi = l.num_groups;  // the last group with no more items before it (one without items has as many as the next)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= item) lo = mid;
+      else hi = mid;
     }
-    before = __builtin_amdgcn_readlane(upto, 63);
+    planned[record] = counts.of_group(l, item, item - before[lo], lo, start[lo], end[lo] - start[lo], shared[lo], per);
   }
-  const int group_items = before;
-  // the sequences' items; every sequence has one at least, which writes down where its rows lie
-  const int item = (wg - group_items) * WAVES + wave;
-  before = 0;
-  latest = latest0;
-  for (int base = 0; base < l.num_seqs; base += 64) {
-    const int b = base + lane;
-    const Own own = base == 0 ? own0 : own_of(base, latest);
-    const int parts = max(1, parts_of(tiles_of(own), per)), items = b < l.num_seqs ? own_blocks * parts : 0;
-    const int upto = before + sum_up_to_lane(items);
-    const uint64_t holds = __ballot(upto > item);
-    if (holds != 0) {
-      const int at = __ffsll((unsigned long long)holds) - 1;
-      const int first = __builtin_amdgcn_readlane(upto - items, at), place = item - first, part = quotient(place, own_blocks);
-      const int from = __builtin_amdgcn_readlane(own.from, at), to = __builtin_amdgcn_readlane(own.to, at), group = __builtin_amdgcn_readlane(own.group, at);
-      const int low = (from / TILE + part * per) * TILE;
-      found.sequence = base + at;
-      found.block = place - part * own_blocks;
-      found.from = max(low, from);
-      found.to = min(low + per * TILE, to);
-      found.at = (group_items << block_shift) + item * 16;
-      found.tells = place == 0;
-      found.rows.own_at = (group_items << block_shift) + first * 16;
-      found.rows.own_parts = __builtin_amdgcn_readlane(parts, at);
-      if (group >= 0) {
-        found.rows.shared_at = (plan.before[group] << block_shift) + (base + at - plan.start[group]) * l.group;
-        found.rows.shared_stride = blocks_of(group) << block_shift;
-        found.rows.shared_parts = parts_of(steps_of(from), per);
-      }
-      return found;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
-  }
-  return found;
+  for (int record = group_items * WAVES + own_items + tid; record < workgroups * WAVES; record += threads) planned[record] = Item{-1, -1, 0, 0, 0, 0, 0, 0};
 }
 
 // ---- rows against a stream of keys ----------------------------------------------------------------------------------------
@@ -686,19 +742,28 @@ template <typename T, int RT> constexpr int workgroups_per_unit() { return D <= 
 // part_o: [KV head][rows_room][D], part_lse: [KV head][rows_room]; directory: [sequence]
 // RT = TALL: rows in blocks of TALL_ROWS over tiles in LDS.
 constexpr int TALL = TALL_ROWS / 16;
+template <typename T> constexpr int tile_shift() { return sizeof(T) == 2 ? 5 : 4; }
+template <typename T, int RT> constexpr int step_shift() { return RT == TALL ? 6 : tile_shift<T>() + 2; }
 template <typename T, int RT>
 __global__ void __launch_bounds__(THREADS, (RT == TALL ? 2 : workgroups_per_unit<T, RT>()))
 shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables, int table_width, const Lengths l, float scale,
                      float* __restrict__ part_o, float* __restrict__ part_lse, Directory* __restrict__ directory) {
-  constexpr int TILE = Block<T>::KB, R = 16 * RT, ROOM = RT == TALL ? 4 * TALL_BYTES : join_bytes<RT>();
-  __shared__ __attribute__((aligned(1024))) char smem[sizeof(Plan) > ROOM ? sizeof(Plan) : ROOM];
+  constexpr int TILE = Block<T>::KB, R = 16 * RT;
+  __shared__ __attribute__((aligned(1024))) char smem[RT == TALL ? 4 * TALL_BYTES : join_bytes<RT>()];
+  __shared__ int begins[THREADS];
   const int kvh = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Item item = find_item<TILE, (RT == TALL ? TALL_TILE : WAVES * TILE)>(l, blockIdx.y, *reinterpret_cast<Plan*>(smem));
+  Item item;
+  if (l.planned != nullptr) {
+    const Item planned = l.planned[blockIdx.y * WAVES + wave];
+    auto of = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    item = Item{of(planned.group), of(planned.sequence), of(planned.first), of(planned.count), of(planned.block), of(planned.from), of(planned.to), of(planned.at)};
+  } else {
+    item = find_item(l, Counts(l, tile_shift<T>(), step_shift<T, RT>()), blockIdx.y, begins + 64 * wave, directory);
+  }
   const int heads = l.group;
   float* const o = part_o + (size_t)kvh * l.rows_room * D;
   float* const lse = part_lse + (size_t)kvh * l.rows_room;
   if (item.group >= 0) {
-    __syncthreads();  // (the plan's place is used again)
     if (item.at + R > l.rows_room) return;  // (groups that overlap: no more than there is room for)
     const int first_row = item.block * R, rows_all = item.count * heads;
     const int* const table = block_tables + (size_t)item.first * table_width;
@@ -720,7 +785,6 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
     return;
   }
   if (item.sequence < 0 || item.at + 16 > l.rows_room) return;
-  if (item.tells && kvh == 0 && lane == 0) directory[item.sequence] = item.rows;
   Rows<T, 1> rows;
   begin_rows<T, 1>(rows, [&](int r) -> const T* {
     const int row = item.block * 16 + r;
@@ -811,13 +875,14 @@ struct SharedPrefixCall {
   const float* sinks;
   void* out;
   float *part_o, *part_lse;
-  int* directory;
+  int *directory, *planned;  // planned: 32 int32 for each of `items`, or nullptr with up to 64 sequences and groups
   long long rows_room;
   int items, qkv_stride, table_width, num_seqs, num_groups, nh, nkv, page_shift, pages, most_keys, row_tiles, target, largest, dtype;
   float scale;
   int unused;
 };
-static_assert(sizeof(SharedPrefixCall) == 13 * 8 + 16 * 4, "as the host packs it");
+static_assert(sizeof(SharedPrefixCall) == 14 * 8 + 16 * 4, "as the host packs it");
+static_assert(sizeof(Item) == 32 && sizeof(Directory) == 32, "as the host counts their room");
 
 template <typename T>
 static int launch(const SharedPrefixCall& c, const Lengths& l, hipStream_t stream) {
@@ -830,6 +895,11 @@ static int launch(const SharedPrefixCall& c, const Lengths& l, hipStream_t strea
   }
   if constexpr (HAS_TALL && sizeof(T) == 2) {
     if (c.row_tiles == TALL) kernel = shared_prefix_kernel<T, TALL>;
+  }
+  if (l.planned != nullptr) {
+    shared_prefix_plan_kernel<<<1, c.num_seqs <= 256 && c.num_groups <= 256 ? 256 : PLAN_THREADS, 0, stream>>>(l, tile_shift<T>(), c.row_tiles == TALL ? step_shift<T, TALL>() : step_shift<T, 1>(), c.items, (Item*)c.planned, directory);
+    const int status = (int)hipGetLastError();
+    if (status != 0) return status;
   }
   kernel<<<dim3(c.nkv, c.items), THREADS, 0, stream>>>((const T*)c.qkv, c.qkv_stride, cache, c.block_tables, c.table_width, l, c.scale, c.part_o, c.part_lse, directory);
   const int status = (int)hipGetLastError();
@@ -850,6 +920,7 @@ extern "C" int velox_shared_prefix_attention(const SharedPrefixCall* call, hipSt
   long long least_items, least_rows;
   velox_shared_prefix_room(c.num_seqs, c.num_groups, group, c.row_tiles, c.target, c.largest, &least_items, &least_rows);
   if (c.items < least_items || c.rows_room < least_rows) return -1;
-  const Lengths l{c.kv_lens, c.group_starts, c.shared_lens, c.num_seqs, c.num_groups, group, 16 * c.row_tiles, c.target, c.most_keys, c.largest, (int)c.rows_room};
+  if (c.planned == nullptr && (c.num_seqs > 64 || c.num_groups > 64)) return -1;
+  const Lengths l{c.kv_lens, c.group_starts, c.shared_lens, (const Item*)c.planned, c.num_seqs, c.num_groups, group, 16 * c.row_tiles, c.target, c.most_keys, c.largest, (int)c.rows_room};
   return c.dtype == VELOX_BF16 ? launch<bf16_t>(c, l, stream) : launch<float>(c, l, stream);
 }

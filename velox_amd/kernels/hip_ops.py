@@ -44,7 +44,7 @@ class _StreamTerms(ctypes.Structure):
                 ("term0_bf16", ctypes.c_int), ("term1_bf16", ctypes.c_int), ("num_terms", ctypes.c_int), ("unused", ctypes.c_int)]
 
 
-_SHARED_PREFIX_CALL = struct.Struct("=13q14ifi")  # ``SharedPrefixCall`` in shared_prefix.hip
+_SHARED_PREFIX_CALL = struct.Struct("=14q14ifi")  # ``SharedPrefixCall`` in shared_prefix.hip
 
 
 class KernelError(RuntimeError):
@@ -2355,7 +2355,8 @@ class HipOps:
         for row_tiles in (1, 2, 8):  # (whichever the largest group asks for)
             blocks, own_blocks = max_num_seqs * group // (16 * row_tiles) + max_num_groups, max_num_seqs * (-(-group // 16))
             rows = max(rows, max(1, 2 * self.num_cus // num_kv_heads) * max(16 * row_tiles, 64) + blocks * 16 * row_tiles + own_blocks * 16 + 64)
-        return rows * num_kv_heads * (head_dim + 1) + 8 * max_num_seqs
+        items = max(1, 2 * self.num_cus // num_kv_heads) + max_num_seqs * group // 16 + max_num_groups + max_num_seqs * (-(-group // 16)) // 4 + 2
+        return rows * num_kv_heads * (head_dim + 1) + 8 * max_num_seqs + 32 * items
 
     def shared_prefix_attention(self, qkv, num_heads, num_kv_heads, head_dim, k_cache, v_cache, block_size, block_tables, kv_lens, group_starts, shared_lens,
                                 largest_group, max_kv_len, scale, workspace, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2414,12 +2415,15 @@ class HipOps:
                                                                     int(max_kv_len))
         if items > 65535:
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
-        # partial outputs, their log-sums, and where each sequence's rows of them lie, eight numbers
+        # partial outputs, their log-sums, where each sequence's rows of them lie, eight numbers, and what each workgroup does, 32 (with up to 64
+        # sequences and groups the workgroups find out for themselves)
         rows_all = rows * num_kv_heads
-        parts = workspace.get("shared_prefix_parts", rows_all * (head_dim + 1) + 8 * num_seqs).data_ptr()
+        ahead = num_seqs > 64 or num_groups > 64
+        parts = workspace.get("shared_prefix_parts", rows_all * (head_dim + 1) + 8 * num_seqs + (32 * items if ahead else 0)).data_ptr()
+        directory = parts + 4 * rows_all * (head_dim + 1)
         call = _SHARED_PREFIX_CALL.pack(
             qkv_at, keys_at, values_at, tables_at, lens_at, starts_at, shared_at, sinks_at, out.data_ptr(), parts, parts + 4 * rows_all * head_dim,
-            parts + 4 * rows_all * (head_dim + 1), rows, items, width, table_width, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages,
+            directory, directory + 32 * num_seqs if ahead else 0, rows, items, width, table_width, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages,
             int(max_kv_len), row_tiles, target, int(largest_group), code, scale, 0)
         self._call("shared_prefix_attention", self.shared_prefix_library(head_dim).velox_shared_prefix_attention, call)
         return out
