@@ -419,12 +419,12 @@ class HipOps:
 
     def _take(self, name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int, ...], align: int = 4) -> int:
         """A tensor's address, after ``_check``'s checks (which speak where one fails)."""
-        if not isinstance(t, torch.Tensor) or t.get_device() != self._index or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-            self._check(name, t, dtype, shape, align)
-        address = t.data_ptr()
-        if address % align != 0:
-            self._check(name, t, dtype, shape, align)
-        return address
+        if isinstance(t, torch.Tensor):
+            address = t.data_ptr()
+            if t.dtype is dtype and t.shape == shape and t.get_device() == self._index and t.is_contiguous() and address % align == 0:
+                return address
+        self._check(name, t, dtype, shape, align)
+        return t.data_ptr()
 
     def _call(self, what: str, function, *args) -> None:
         """Launches with the kernels' device as the current one (a launch goes to the current device's queues)."""
