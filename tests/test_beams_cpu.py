@@ -101,7 +101,7 @@ def test_attention_items_are_enough(ops, heads, kv_heads, dim):
         num_seqs = max(1, sum(sizes) + rng.randint(0, 5))
         element_size = rng.choice([2, 4])
         tile = 32 if element_size == 2 else 16
-        row_tiles, target, items, rows = ops._shared_prefix_shape(256, num_seqs, len(sizes), heads, kv_heads, dim, element_size, max(sizes + [1]), rng.choice([100, 40000]))
+        row_tiles, target, items, rows = ops._shared_prefix_shape(256, num_seqs, len(sizes), heads, kv_heads, dim, element_size, max(sizes + [1]), rng.choice([1100, 40000]))
         own_blocks = -(-group // 16)
         shared_work, own_work = [], []  # (row blocks, steps) of the groups, tiles of the sequences
         for size in sizes:

@@ -44,7 +44,7 @@ class Batch:
             shared.append(keys)
         num = starts[-1] + behind
         assert len(lens) == num
-        width = max(1, -(-max(lens) // page)) + 1
+        width = max(-(-max(lens) // page), 1050 // page) + 1
         wild = 0
         tables = torch.full((num, width), wild, dtype=torch.int32)
         pages = 1 + sum(-(-n // page) for n in lens) + 3
@@ -71,7 +71,8 @@ class Batch:
         self.tables, self.lens = tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
         self.starts, self.shared = torch.tensor(starts, dtype=torch.int32).cuda(), torch.tensor(shared, dtype=torch.int32).cuda()
         self.largest = max([c for c, _ in groups], default=1)
-        self.longest = max(lens)
+        self.most_keys = max(lens)
+        self.longest = max(max(lens), 1050)  # (keys enough to be shared out among workgroups)
         self.scale = dim ** -0.5
         self.sinks = torch.randn(heads, generator=g).cuda() if sinks else None
 
@@ -87,7 +88,7 @@ class Batch:
         # argument by 2^-24 of it each; a relative error of the weights twice that (numerator and denominator).  Exponentials and sums of up to
         # n weights or weighted values, joined once: (n + 64) 2^-24, and 2^-21 for each of exp (two, the joining's among them).  In bfloat16 a weight is
         # rounded before its product (2^-8 of the values' magnitudes) and so is the result (2^-8 of it); float32 results by 2^-24.
-        n = max(self.longest, 1)
+        n = max(self.most_keys, 1)
         weights = 2 * (dim + 4) * 2.0 ** -24 * reach[:, :, None] + (n + 64) * 2.0 ** -24 + 2 * 2.0 ** -21
         rounding = 2.0 ** -8 if self.qkv.dtype == BF16 else 2.0 ** -24
         allowed = size * (weights + (2.0 ** -8 if self.qkv.dtype == BF16 else 0)) * 1.01 + rounding * want.abs() * 1.01 + 1e-30
@@ -249,6 +250,42 @@ def test_attention_result_does_not_hang_on_the_bounds(ops, workspace):
     b.check(b.run(ops, workspace, largest=4, longest=b.tables.shape[1] * 16))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shared", [1, 31, 32, 33, 64, 129, 200])
+def test_attention_few_keys(ops, workspace, dtype, shape, shared):
+    """A workgroup takes all of a sequence's keys."""
+    lens = [37, 1, 0] + own(5, shared, 0, 50) + own(3, 64, 1, 40) + [min(shared, 20), 130]
+    b = Batch(dtype, *shape, groups=[(5, shared), (4, 64)], lens=lens, before=3, behind=1, sinks=shared % 2 == 1)
+    assert ops._shared_prefix_shape(ops.num_cus, 13, 2, *shape[:3], 4 if dtype == F32 else 2, 5, b.most_keys)[0] == 0
+    for largest in (5, 13):
+        b.check(b.run(ops, workspace, largest=largest, longest=b.most_keys))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_few_keys_of_many_groups(ops, workspace, dtype):
+    sizes = [(1 + g % 3, 3 + 5 * (g % 7)) for g in range(200)]
+    lens = [length for g, (count, shared) in enumerate(sizes) for length in own(count, shared, g % 2, 30)]
+    b = Batch(dtype, 4, 2, 64, 16, groups=sizes, lens=lens)
+    assert ops._shared_prefix_shape(ops.num_cus, len(lens), 200, 4, 2, 64, 4 if dtype == F32 else 2, 3, b.most_keys)[0] == 0
+    b.check(b.run(ops, workspace, longest=b.most_keys))
+    b.check(b.run(ops, workspace))
+
+
+def test_attention_few_keys_of_a_group_larger_than_said(ops, workspace):
+    """What a group has beyond the largest reads its own pages alone."""
+    b = Batch(BF16, 12, 2, 128, 16, groups=[(6, 100)], lens=own(6, 100, 1, 60))
+    b.tables[4:, :100 // 16] = b.tables[0, :100 // 16]  # (their own tables lead to the shared keys as well)
+    last = b.tables[4:, 100 // 16].tolist()
+    for page in last:
+        b.k[page, :, :100 % 16] = b.k[b.tables[0, 100 // 16], :, :100 % 16]
+        b.v[page, :, :, :100 % 16] = b.v[b.tables[0, 100 // 16], :, :, :100 % 16]
+    want = b.run(ops, workspace, longest=b.most_keys)
+    b.check(want)
+    assert torch.equal(b.run(ops, workspace, largest=4, longest=b.most_keys)[:4], want[:4])
+    b.check(b.run(ops, workspace, largest=4, longest=b.most_keys))
+
+
 def test_attention_group_larger_than_said(ops, workspace):
     """What a group has beyond ``largest_group`` reads all its keys through its own table."""
     b = Batch(BF16, 12, 2, 128, 16, groups=[(4, 0), (5, 0)], lens=own(4, 450, 1, 50) + own(5, 90, 1, 50))
@@ -281,12 +318,12 @@ def test_attention_agrees_with_paged_attention(ops, workspace):
     torch.testing.assert_close(got.float(), want.float(), rtol=2 * 2.0 ** -8, atol=2 * 2.0 ** -8)
 
 
-def test_attention_captured(ops):
+@pytest.mark.parametrize("most", [256, 1050])
+def test_attention_captured(ops, most):
     """A captured call replays with other lengths, other groups and other pages' contents, with eager calls of the same workspace between."""
     workspace = Workspace(torch.device("cuda"))
     a = Batch(F32, 8, 2, 64, 16, groups=[(3, 200), (2, 70)], lens=own(3, 200, 1, 60) + own(2, 70, 1, 50), seed=1)
-    other = Batch(F32, 8, 2, 64, 16, groups=[(2, 100), (3, 33)], lens=own(2, 100, 1, 160) + own(3, 33, 1, 220), seed=2)
-    most = max(a.longest, other.longest)
+    other = Batch(F32, 8, 2, 64, 16, groups=[(2, 100), (3, 33)], lens=own(2, 100, 1, 150) + own(3, 33, 1, 220), seed=2)
     width = max(a.tables.shape[1], other.tables.shape[1])
     pages = max(a.k.shape[0], other.k.shape[0])
     for b in (a, other):

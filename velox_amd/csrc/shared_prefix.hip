@@ -507,10 +507,11 @@ template <typename T, int RT> __device__ __forceinline__ void finish_sums(Rows<T
   }
 }
 
-// The four waves' results of the same rows, put together and written to part_o[row][D] and part_lse[row] (the first `count` rows), a row tile at a time.
+// The four waves' results of the same rows, put together a row tile at a time.  `scaled(row, top, total)`: what its sums of weighted values are multiplied by,
+// given the exponents' reference (natural units) and the sum of weights; `leave(row, channel, four)`.
 template <int RT> constexpr int join_bytes() { return WAVES * (D / 16) * 64 * 16 + 2 * WAVES * 16 * RT * 4; }
-template <typename T, int RT>
-__device__ __forceinline__ void join_waves(Rows<T, RT>& rows, int count, float* __restrict__ part_o, float* __restrict__ part_lse, char* smem) {
+template <typename T, int RT, typename Scaled, typename Leave>
+__device__ __forceinline__ void join_waves(Rows<T, RT>& rows, int count, char* smem, Scaled scaled, Leave leave) {
   typedef Block<T> B;
   constexpr int NC = D / 16;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -542,14 +543,14 @@ __device__ __forceinline__ void join_waves(Rows<T, RT>& rows, int count, float* 
       weight[w] = m == -INFINITY ? 0.f : B::exp_of(m - safe);
       total += weight[w] * l_all[w * 16 * RT + 16 * rt + i];
     }
-    const float inv = total > 0.f ? 1.f / total : 1.f;
+    const bool there = 16 * rt + i < count;
+    const float by = there ? scaled(16 * rt + i, top * B::LN_UNIT, total) : 0.f;
     for (int c = wave; c < NC; c += WAVES) {
       float4_t sum = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) sum += acc_all[(w * NC + c) * 64 + lane] * weight[w];
-      if (16 * rt + i < count) *reinterpret_cast<float4_t*>(part_o + (size_t)(16 * rt + i) * D + 16 * c + 4 * g) = sum * inv;
+      if (there) leave(16 * rt + i, 16 * c + 4 * g, sum * by);
     }
-    if (wave == 0 && g == 0 && 16 * rt + i < count) part_lse[16 * rt + i] = total > 0.f ? top * B::LN_UNIT + logf(total) : -INFINITY;
   }
 }
 
@@ -780,7 +781,12 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
       Rows<T, RT> rows;
       begin_rows<T, RT>(rows, [&](int r) { return query_of(first_row + r); });
       stream_keys<T, RT>(rows, cache, kvh, table, item.from, item.to, item.from / TILE + wave, WAVES, scale);
-      join_waves<T, RT>(rows, rows_all - first_row, o + (size_t)item.at * D, lse + item.at, smem);
+      join_waves<T, RT>(rows, rows_all - first_row, smem,
+                        [&](int row, float top, float total) {
+                          if (wave == 0 && lane < 16) lse[item.at + row] = total > 0.f ? top + logf(total) : -INFINITY;
+                          return total > 0.f ? 1.f / total : 1.f;
+                        },
+                        [&](int row, int channel, const float4_t& four) { *reinterpret_cast<float4_t*>(o + (size_t)(item.at + row) * D + channel) = four; });
     }
     return;
   }
@@ -793,6 +799,50 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
   if (item.to > item.from)
     stream_keys<T, 1>(rows, cache, kvh, block_tables + (size_t)item.sequence * table_width, item.from, item.to, item.from / TILE, 1, scale);
   leave_rows<T, 1>(rows, heads - 16 * item.block, o + (size_t)item.at * D, lse + item.at);
+}
+
+// Few keys: a workgroup per (KV head, sequence, 16 of its rows) takes all of them, the shared ones too, and leaves the result itself: no plan, no parts, nothing to join.
+template <typename T>
+__global__ void __launch_bounds__(THREADS, (workgroups_per_unit<T, 1>()))
+shared_prefix_direct_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables, int table_width, const Lengths l, float scale,
+                            const float* __restrict__ sinks, T* __restrict__ out) {
+  constexpr int TILE = Block<T>::KB;
+  __shared__ __attribute__((aligned(16))) char smem[join_bytes<1>()];
+  const int kvh = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = l.group, first_row = 16 * blockIdx.z, len = clamped(l.kv_lens[b], 0, l.most);
+  int first = b, shared = 0;
+  for (int base = 0; base < l.num_groups; base += 64) {
+    const int g = min(base + lane, l.num_groups - 1);
+    const int start = clamped(l.group_starts[g], 0, l.num_seqs), end = clamped(l.group_starts[g + 1], start, min(l.num_seqs, start + l.largest)), keys = l.shared_lens[g];
+    const uint64_t holds = __ballot(base + lane < l.num_groups && start <= b && b < end && end - start > 1);
+    if (holds != 0) {
+      const int at = 63 - __builtin_clzll(holds);
+      first = __builtin_amdgcn_readlane(start, at);
+      shared = __builtin_amdgcn_readlane(keys, at);
+    }
+  }
+  shared = clamped(shared, 0, first == b ? len : clamped(l.kv_lens[first], 0, l.most));
+  if (shared > len) shared = 0;
+  Rows<T, 1> rows;
+  begin_rows<T, 1>(rows, [&](int r) -> const T* {
+    return first_row + r < heads ? qkv + (size_t)b * qkv_stride + (size_t)(kvh * heads + first_row + r) * D : nullptr;
+  });
+  // (a sequence's own tiles begin with the wave that the shared ones end before)
+  const int shared_tiles = (shared + TILE - 1) / TILE;
+  if (shared > 0) stream_keys<T, 1>(rows, cache, kvh, block_tables + (size_t)first * table_width, 0, shared, wave, WAVES, scale);
+  if (len > shared)
+    stream_keys<T, 1>(rows, cache, kvh, block_tables + (size_t)b * table_width, shared, len, shared / TILE + ((wave - shared_tiles) & (WAVES - 1)), WAVES, scale);
+  T* const to = out + ((size_t)b * l.group * cache.nkv + kvh * heads + first_row) * D;
+  join_waves<T, 1>(rows, heads - first_row, smem,
+                   [&](int row, float top, float total) {
+                     if (total <= 0.f) return 1.f;
+                     return 1.f / (total + (sinks != nullptr ? expf(sinks[kvh * heads + first_row + row] - top) : 0.f));
+                   },
+                   [&](int row, int channel, const float4_t& four) {
+                     T* const dst = to + (size_t)row * D + channel;
+#pragma unroll
+                     for (int j = 0; j < 4; ++j) dst[j] = from_f32<T>(four[j]);
+                   });
 }
 
 // A wave per (head, sequence): the parts that hold its row, joined.  Lane p asks for part p's log-sum (the next 64 parts', if there are more, in
@@ -888,6 +938,11 @@ template <typename T>
 static int launch(const SharedPrefixCall& c, const Lengths& l, hipStream_t stream) {
   const Cache<T> cache{(const T*)c.k_cache, (const T*)c.v_cache, c.nkv, c.page_shift, (uint32_t)(c.pages - 1)};
   constexpr int MOST = most_row_tiles<T>();
+  if (c.row_tiles == 0) {
+    shared_prefix_direct_kernel<T><<<dim3(c.nkv, c.num_seqs, (l.group + 15) / 16), THREADS, 0, stream>>>((const T*)c.qkv, c.qkv_stride, cache, c.block_tables, c.table_width, l, c.scale,
+                                                                                                  c.sinks, (T*)c.out);
+    return (int)hipGetLastError();
+  }
   Directory* const directory = (Directory*)c.directory;
   auto kernel = shared_prefix_kernel<T, 1>;
   if constexpr (MOST >= 2) {
@@ -914,13 +969,15 @@ extern "C" int velox_shared_prefix_attention(const SharedPrefixCall* call, hipSt
   if (c.num_seqs <= 0) return 0;
   if (c.nkv < 1 || c.nh < 1 || c.nh % c.nkv != 0 || c.page_shift < 3 || c.page_shift > 16 || c.pages < 1 || c.most_keys < 0 || c.most_keys > MOST_KEYS || c.most_keys > (long long)c.table_width << c.page_shift ||
       c.num_groups < 0 || c.num_groups > MOST_GROUPS || c.target < 1 || c.largest < 1 || c.largest > c.num_seqs || c.num_seqs > 65535 || c.items > 65535 || c.rows_room > 0x7fffffffLL) return -1;
-  if (c.row_tiles < 1 || (c.row_tiles & (c.row_tiles - 1)) != 0 ||
+  if (c.row_tiles < 0 || (c.row_tiles & (c.row_tiles - 1)) != 0 ||
       (c.row_tiles > velox_shared_prefix_most_row_tiles(c.dtype) && c.row_tiles != velox_shared_prefix_tall(c.dtype))) return -1;
   const int group = c.nh / c.nkv;
-  long long least_items, least_rows;
-  velox_shared_prefix_room(c.num_seqs, c.num_groups, group, c.row_tiles, c.target, c.largest, &least_items, &least_rows);
-  if (c.items < least_items || c.rows_room < least_rows) return -1;
-  if (c.planned == nullptr && (c.num_seqs > 64 || c.num_groups > 64)) return -1;
+  if (c.row_tiles > 0) {
+    long long least_items, least_rows;
+    velox_shared_prefix_room(c.num_seqs, c.num_groups, group, c.row_tiles, c.target, c.largest, &least_items, &least_rows);
+    if (c.items < least_items || c.rows_room < least_rows) return -1;
+    if (c.planned == nullptr && (c.num_seqs > 64 || c.num_groups > 64)) return -1;
+  }
   const Lengths l{c.kv_lens, c.group_starts, c.shared_lens, (const Item*)c.planned, c.num_seqs, c.num_groups, group, 16 * c.row_tiles, c.target, c.most_keys, c.largest, (int)c.rows_room};
   return c.dtype == VELOX_BF16 ? launch<bf16_t>(c, l, stream) : launch<float>(c, l, stream);
 }

@@ -2328,6 +2328,10 @@ class HipOps:
         """Row tiles of a workgroup, over how many workgroups per KV head the keys are cut, and how many workgroups and rows of partial results
         per KV head that makes at most (as ``velox_shared_prefix_room`` counts them).
 
+        Few keys are not shared out at all: no row tiles (0), a workgroup per sequence, KV head and 16 rows takes all of its keys.  Measured on MI355X (us; shared
+        out / not, a quarter of the keys each sequence's own): 4 sequences of 256 bfloat16 keys (12 heads over 2) 9.6 / 6.7, of 512 9.7 / 8.8, 1,024 11.4 / 13.3; 64 of 512
+        (28 over 4) 13.3 / 11.3, 1,024 15.6 / 16.0; 240 (960 workgroups) of 256 23.9 / 20.7, 512 28.6 / 29.6; 240 (1,920) of 128 18.7 / 13.0, 512 24.4 / 27.8.  In float32 4 of 256
+        12.3 / 10.5, 512 14.0 / 16.5; 240 (960) of 128 27.5 / 25.1, 256 33.6 / 35.4.
         Row tiles go by the rows of the largest group: one or two of 16, or eight with tiles of keys in LDS (8).  Measured on MI355X (us, both kernels; 28 heads
         over 4, one group): two / eight with 84 rows behind 8,192 keys 17.2 / 31.5, 224 22.7 / 23.9 and behind 32,768 52 / 49, 336 behind 8,192 33.7 / 28.1, behind 32,768
         102 / 57, 448 behind 1,024 15.6 / 21.0, 4,096 25.2 / 24.8, 32,768 111 / 65; 320 of 64 channels behind 2,048 16.9 / 18.8, 16,384 44.8 / 37.8.  In float32 matrix
@@ -2335,6 +2339,8 @@ class HipOps:
         A workgroup per compute unit but where rows are many or float32 ones are in single tiles, two: one / two with 8 groups of 4 behind 1,024 to 2,048 keys 16.0 / 25.2
         (more parts to join), 140 rows behind 8,192 19.7 / 22.0; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
         group = num_heads // num_kv_heads
+        if max_kv_len * element_size * max(num_seqs * num_kv_heads * (-(-group // 16)), 2 * num_cus) <= 2048 * num_cus:
+            return 0, 1, 0, 0
         rows = largest_group * group
         row_tiles, per_unit = 1 if rows <= 16 or head_dim > 128 else 2, 1
         if element_size == 2 and head_dim in (64, 128) and rows > 256 and max_kv_len >= 4096:
@@ -2415,15 +2421,19 @@ class HipOps:
                                                                     int(max_kv_len))
         if items > 65535:
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
-        # partial outputs, their log-sums, where each sequence's rows of them lie, eight numbers, and what each workgroup does, 32 (with up to 64
-        # sequences and groups the workgroups find out for themselves)
-        rows_all = rows * num_kv_heads
-        ahead = num_seqs > 64 or num_groups > 64
-        parts = workspace.get("shared_prefix_parts", rows_all * (head_dim + 1) + 8 * num_seqs + (32 * items if ahead else 0)).data_ptr()
-        directory = parts + 4 * rows_all * (head_dim + 1)
+        directory = parts = planned = sums = 0
+        if row_tiles > 0:
+            # partial outputs, their log-sums, where each sequence's rows of them lie, eight numbers, and what each workgroup does, 32 (with up to
+            # 64 sequences and groups the workgroups find out for themselves)
+            rows_all = rows * num_kv_heads
+            ahead = num_seqs > 64 or num_groups > 64
+            parts = workspace.get("shared_prefix_parts", rows_all * (head_dim + 1) + 8 * num_seqs + (32 * items if ahead else 0)).data_ptr()
+            sums = parts + 4 * rows_all * head_dim
+            directory = sums + 4 * rows_all
+            planned = directory + 32 * num_seqs if ahead else 0
         call = _SHARED_PREFIX_CALL.pack(
-            qkv_at, keys_at, values_at, tables_at, lens_at, starts_at, shared_at, sinks_at, out.data_ptr(), parts, parts + 4 * rows_all * head_dim,
-            directory, directory + 32 * num_seqs if ahead else 0, rows, items, width, table_width, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages,
+            qkv_at, keys_at, values_at, tables_at, lens_at, starts_at, shared_at, sinks_at, out.data_ptr(), parts, sums, directory, planned,
+            rows, items, width, table_width, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages,
             int(max_kv_len), row_tiles, target, int(largest_group), code, scale, 0)
         self._call("shared_prefix_attention", self.shared_prefix_library(head_dim).velox_shared_prefix_attention, call)
         return out
