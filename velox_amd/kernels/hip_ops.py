@@ -2439,10 +2439,11 @@ class HipOps:
         return out
 
     def _beam_pieces(self, rows: int, vocab: int) -> int:
-        """Into how many pieces ``beam_select`` cuts a row: as many as give the compute units two and a half workgroups each, of 2,048 tokens at least.
-        Measured on MI355X (us, the kernel that reads the logits): 512 rows of 152,064 whole 100, in 2 pieces 83, in 4 86; 64 rows in 4 25.0, in 8
-        19.7, in 16 21.1; 168 rows of 32,003 in 2 19.7, in 4 16.8, in 8 20.5."""
-        return max(1, min(-(-5 * self.num_cus // (2 * rows)), -(-vocab // 2048)))
+        """Into how many pieces ``beam_select`` cuts a row: as many as give the compute units two and a half workgroups each, of 4,096 tokens at least, or
+        up to four of 2,048.  Measured on MI355X (us, the kernel that reads the logits): 512 rows of 152,064 whole 100, in 2 pieces 83, in 4 86; 64 rows in 4
+        25.0, in 8 19.7, in 16 21.1; 168 rows of 32,003 in 2 19.7, in 4 16.8, in 8 20.5.  Both kernels (more pieces, more to join): 4 rows of 151,936 in 24 15.7,
+        in 38 14.6, in 75 16.2; 8 of 32,000 in 4 16.0, in 8 14.7, in 16 14.9; 12 of 7,847 in 1 13.9, in 2 11.7, in 4 11.0."""
+        return max(1, min(-(-5 * self.num_cus // (2 * rows)), max(-(-vocab // 4096), min(4, -(-vocab // 2048)))))
 
     def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, keep: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """The ``keep`` best continuations of every request over its beams and the vocabulary.  ``logits`` float32 ``[requests * beams, vocab]``,
