@@ -10,11 +10,23 @@
 // are the same for the group's sequences, so n_g G rows of queries stand against one stream of keys and values, which is read
 // once; the second part is each sequence's own, G rows against its keys.
 //
-// Both parts are cut into items of about equally many keys (see `Plan`), all in one launch; a second kernel joins what the items leave.
+// Four kernels; which ones a call takes goes by its sizes (the host's rules):
+//
+//   few keys        a workgroup per (KV head, sequence, 16 rows) takes all of its keys, nothing is shared out (shared_prefix_direct_kernel)
+//   else            both parts are cut into items of about equally many keys, all in one launch, and a second kernel joins what the items leave;
+//                   with more than 64 sequences or groups a third one has worked the items out before
+//
 // A group's item is a workgroup's: its four waves take a tile of keys in turn, each straight from the cache into the operands of matrix
 // instructions, and put their results together at the end.  A sequence's own keys are single waves' items, four of them to a workgroup.  No
 // wave shares a key with another, so nothing is staged and no barrier stands in the loop: the next tile's keys are asked for as soon as
-// this one's have been multiplied, its values as soon as this one's have, two workgroups to a compute unit.
+// this one's have been multiplied, its values as soon as this one's have, two workgroups to a compute unit.  With many rows the products
+// count, and the waves share tiles in LDS instead (tall_item).
+//
+// What bounds them, measured on MI355X (bfloat16, main + joining kernel alone): 48 groups of 5 behind 700 keys (32 heads over 8 of 64 channels, 76 MB) 4.7 + 18.5 +
+// 5.0 us, the stream at 4.1 TB/s in the main one, 2.8 of all three; 8 groups of up to 4 behind 2,048 (28 over 4 of 128, 31 MB) 11.9 + 4.3, four loads that
+// wait for one another and two launches; 64 sequences behind 8,192 (28 over 4, 7.6 GFLOP) 23.4 + 6.5, of which writing and reading the parts' 2 x 24 MB is 8 and
+// half a tile of rows is padding; behind 32,768 (40 over 8, 43 GFLOP) 84.6 to 90 + 8, 0.5 PFLOP/s: exponentials and matrix instructions of two waves a SIMD
+// in turn, at the clock the card holds under them.  4 sequences of 321 keys, taken whole, 8.0 us, in parts it was 7.4 + 3.2 and a launch more.
 //
 // Matrix cores: S^T[key, row] = K Q^T and O^T[channel, row] = V^T P^T, both with 16 x 16 results.  For a block of KB contraction
 // indices (32 in bfloat16, 16 in float32) lane (g = lane / 16, i = lane % 16) holds 16 bytes of row or column i, those of place g; a result is rows
@@ -73,9 +85,10 @@ template <> struct Block<float> {
 // ---- which workgroup does what -----------------------------------------------------------------------------------------
 // Everything is worked out from the lengths on the device, so that a captured step replays with other lengths.  A group's shared
 // keys are those of its first sequence at most (it is through that one's table that they are read); a sequence with fewer keys
-// than its group shares, one that is alone in its group or in none, and what a group has beyond `largest` share nothing.  A step is a tile of keys for each of four waves; all
-// items' steps over `target` workgroups are what one item may have (`per`: of a sequence's own keys, tiles of one wave).  A group's rows are cut
-// into blocks of `block_rows`, a sequence's G rows into blocks of 16.
+// than its group shares, one that is alone in its group or in none, and what a group has beyond `largest` share nothing.  A step is a tile of
+// keys for each of four waves (with many rows: one of the tiles that they share); all items' steps over `target` workgroups are what one item
+// may have (`per`: of a sequence's own keys, tiles of one wave).  A group's rows are cut into blocks of `block_rows`, a sequence's G rows into
+// blocks of 16.
 //
 // What the items leave has rows of its own, per KV head: `block_rows` for every item of a group, in the order groups, parts of the keys, row blocks, then
 // 16 for every item of a sequence, in the order sequences, parts, blocks.  Row r of a group's or of a sequence's part p then lies at
@@ -214,7 +227,7 @@ __device__ __forceinline__ Item find_item(const Lengths& l, const Counts& counts
   return counts.of_sequence(item, item - first, at, from, of(own.to, at), per, group_items);
 }
 
-// With more of either a workgroup ahead works all items out: a thread has a group and a sequence of its own (of these as many at a time), then every item is
+// With more of either a workgroup ahead works all items out (240 sequences 4.6 us, 1,000 6.5): a thread has a group and a sequence of its own (of these as many at a time), then every item is
 // looked up by halving.  planned: [workgroup][wave], a group's item four times.
 constexpr int PLAN_THREADS = 1024;
 static_assert(MOST_GROUPS <= PLAN_THREADS, "a thread has a group");
@@ -556,7 +569,8 @@ __device__ __forceinline__ void join_waves(Rows<T, RT>& rows, int count, char* s
 
 // ---- many rows: tiles in LDS ------------------------------------------------------------------------------------------------------
 // `idle`: the wave has no rows and only brings tiles.
-// From some hundred rows on the products count, and every 32 rows reading the keys for themselves is more than the second-level caches give.  Here the four
+// From some hundred rows on the products count, and every 32 rows reading the keys for themselves is more than the second-level caches give (448 rows behind 32,768 keys, 28
+// heads over 4: 111 us that way, 65 this way).  Here the four
 // waves have 32 rows each and share tiles of 64 keys (bfloat16, heads of 64 and 128 channels).  Every lane asks for 16 bytes of the cache with a
 // load that writes LDS itself, a whole tile ahead of the one being multiplied, into the other of two buffers; one barrier a tile is left.  Such a load fills
 // a contiguous kilobyte, so what lies where is decided by which piece each lane asks for: pieces of 16 bytes change places within a
@@ -801,7 +815,9 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
   leave_rows<T, 1>(rows, heads - 16 * item.block, o + (size_t)item.at * D, lse + item.at);
 }
 
-// Few keys: a workgroup per (KV head, sequence, 16 of its rows) takes all of them, the shared ones too, and leaves the result itself: no plan, no parts, nothing to join.
+// Few keys: a workgroup per (KV head, sequence, 16 of its rows) takes all of them, the shared ones too, and leaves the result itself: no plan, no parts, nothing to
+// join.  What bounds it is latency: a launch (1.6 us), lengths, page ids and keys that wait for one another (0.8 us each), then about 0.7 us for each of a
+// wave's tiles; 4 sequences of 321 keys (12 heads over 2) take 8.0 us.  (With how many keys sharing them out is better: see the host's rule.)
 template <typename T>
 __global__ void __launch_bounds__(THREADS, (workgroups_per_unit<T, 1>()))
 shared_prefix_direct_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables, int table_width, const Lengths l, float scale,
@@ -847,7 +863,7 @@ shared_prefix_direct_kernel(const T* __restrict__ qkv, int qkv_stride, const Cac
 
 // A wave per (head, sequence): the parts that hold its row, joined.  Lane p asks for part p's log-sum (the next 64 parts', if there are more, in
 // another round) and every lane for its own channels of up to AHEAD parts, all before it waits for any of them.  A sink adds exp(sink) to the
-// denominator.
+// denominator.  (About 4 us for small calls: a launch and three loads in a row; 64 sequences of 28 heads with 27 parts 6.5 us, 24 MB at 3.7 TB/s.)
 constexpr int LANE_CHANNELS = D <= 64 ? 1 : D <= 128 ? 2 : 4, JOIN_HEADS = 4;
 template <typename T>
 __global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int nh, int group, int rows_room, const Directory* __restrict__ directory,
