@@ -357,6 +357,46 @@ def test_attention_captured(ops, most):
             b.check(result.clone())
 
 
+def test_attention_captured_of_many_sequences(ops):
+    """Two captured calls that share a workspace, planned ahead, replayed in turn with other lengths and groups, eager calls between."""
+    workspace = Workspace(torch.device("cuda"))
+    made = []
+    for count, dtype in ((70, BF16), (90, F32)):
+        most = 400
+        groups = [(5, 100 + 3 * g) for g in range(count // 5)]
+        first = Batch(dtype, 8, 2, 64, 16, groups=groups, lens=[n for g in range(count // 5) for n in own(5, 100 + 3 * g, 1, 60)])
+        second = Batch(dtype, 8, 2, 64, 16, groups=groups[:-1] + [(5, 0)], lens=[n for g in range(count // 5) for n in own(5, 100 + 3 * g, 0, 40)], seed=3)
+        live = {name: getattr(first, name).clone() for name in ("qkv", "tables", "lens", "starts", "shared")}
+        pages = max(first.k.shape[0], second.k.shape[0])
+        for b in (first, second):
+            spare = pages - b.k.shape[0]
+            b.k, b.v = (torch.cat([t, torch.full_like(t[:1], math.nan).expand(spare, -1, -1, -1)]) if spare else t for t in (b.k, b.v))
+        live["k"], live["v"] = first.k.clone(), first.v.clone()
+
+        def call(live=live, args=first.args, scale=first.scale, largest=first.largest):
+            return ops.shared_prefix_attention(live["qkv"], *args, live["k"], live["v"], 16, live["tables"], live["lens"], live["starts"], live["shared"], largest, 1050, scale, workspace)
+
+        made.append([first, second, live, call])
+    for _, _, _, call in made:
+        call()
+    torch.cuda.synchronize()
+    for m in made:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            m.append(m[3]())
+        m.append(graph)
+    for round in range(4):
+        for first, second, live, call, result, graph in made:
+            b = (first, second)[round % 2]
+            for name, t in live.items():
+                t.copy_(getattr(b, name))
+            graph.replay()
+            eager = call()
+            torch.cuda.synchronize()
+            assert torch.equal(result, eager)
+            b.check(eager)
+
+
 def test_attention_on_another_stream(ops, workspace):
     b = Batch(BF16, 12, 2, 128, 16, groups=[(6, 700)], lens=own(6, 700, 1, 200))
     want = b.run(ops, workspace)

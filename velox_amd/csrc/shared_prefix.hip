@@ -324,12 +324,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_prefix_plan_kernel(const 
         if (upto[mid] > t) hi = mid;
         else lo = mid;
       }
-      const int item = own_items + t, record = group_items * WAVES + item;
+      const int item = own_items + t, record = min(group_items, workgroups) * WAVES + item;  // (groups that overlap may have more)
       if (record < workgroups * WAVES) planned[record] = counts.of_sequence(item, t - (hi > 0 ? upto[hi - 1] : 0), base + hi, from[hi], to[hi], per, group_items);
     }
     own_items += sums.all_own;
   }
-  for (int record = tid; record < group_items * WAVES && record < workgroups * WAVES; record += threads) {
+  const int group_records = min(group_items, workgroups) * WAVES;
+  for (int record = tid; record < group_records; record += threads) {
     const int item = record / WAVES;
     int lo = 0, hi = l.num_groups;  // the last group with no more items before it (one without items has as many as the next)
     while (hi - lo > 1) {
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_prefix_plan_kernel(const 
     }
     planned[record] = counts.of_group(l, item, item - before[lo], lo, start[lo], end[lo] - start[lo], shared[lo], per);
   }
-  for (int record = group_items * WAVES + own_items + tid; record < workgroups * WAVES; record += threads) planned[record] = Item{-1, -1, 0, 0, 0, 0, 0, 0};
+  for (int record = group_records + own_items + tid; record < workgroups * WAVES; record += threads) planned[record] = Item{-1, -1, 0, 0, 0, 0, 0, 0};
 }
 
 // ---- rows against a stream of keys ----------------------------------------------------------------------------------------

@@ -2338,6 +2338,11 @@ class HipOps:
         instructions decide and padded rows cost: one / two row tiles with 48 rows 16.7 / 19.7, 112 37.8 / 40.9, 28 32.3 / 31.2.
         A workgroup per compute unit but where rows are many or float32 ones are in single tiles, two: one / two with 8 groups of 4 behind 1,024 to 2,048 keys 16.0 / 25.2
         (more parts to join), 140 rows behind 8,192 19.7 / 22.0; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
+        def refuse():
+            raise KernelError(f"shared_prefix_attention: {num_seqs} sequences of up to {max_kv_len} keys are more than one call takes")
+
+        if num_seqs > 65535:
+            refuse()
         group = num_heads // num_kv_heads
         if max_kv_len * element_size * max(num_seqs * num_kv_heads * (-(-group // 16)), 2 * num_cus) <= 2048 * num_cus:
             return 0, 1, 0, 0
@@ -2350,8 +2355,8 @@ class HipOps:
         target = max(1, per_unit * num_cus // num_kv_heads)
         block_rows, own_blocks = 16 * row_tiles, num_seqs * (-(-group // 16))
         blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-rows // block_rows))
-        if (own_blocks + blocks) * (max_kv_len // 16 + 2) > 0x7FFFFFFF or num_seqs > 65535:  # (tiles of keys are counted in 32 bits)
-            raise KernelError(f"shared_prefix_attention: {num_seqs} sequences of up to {max_kv_len} keys are more than one call takes")
+        if (own_blocks + blocks) * (max_kv_len // 16 + 2) > 0x7FFFFFFF:  # (tiles of keys are counted in 32 bits)
+            refuse()
         return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
 
     def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> int:
