@@ -625,19 +625,27 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
   const int value_first = value_row + 64 * half, value_second = value_row + 64 * (1 - half);
   const float scale_eff = scale * B::SCALE;
 
+  // Operands are read a few products ahead, in this order: left to the compiler, which has no registers to spare here, most were read right before their
+  // product, and its wait was longer than the product (one group behind 32,768 keys 86 us, this way 82).
+  constexpr int KEYS_AHEAD = 6, VALUES_AHEAD = 3;
   auto multiply_keys = [&](float4_t (&s)[CT][NT], const char* tile) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float4_t k[NQB];
-#pragma unroll
-      for (int cb = 0; cb < NQB; ++cb)
-        k[cb] = *reinterpret_cast<const float4_t*>(tile + ((cb & 1) ? key_odd : key_even) + 128 * (cb >> 1) + (32 * (t >> 1) + 4 * (t & 1)) * (2 * D));
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) s[ct][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+    float4_t k[KEYS_AHEAD];
+    auto read = [&](int e) {  // contraction block e % NQB of score tile e / NQB
+      const int t = e / NQB, cb = e % NQB;
+      k[e % KEYS_AHEAD] = *reinterpret_cast<const float4_t*>(tile + ((cb & 1) ? key_odd : key_even) + 128 * (cb >> 1) + (32 * (t >> 1) + 4 * (t & 1)) * (2 * D));
+    };
 #pragma unroll
-      for (int cb = 0; cb < NQB; ++cb)
+    for (int e = 0; e < KEYS_AHEAD - 1; ++e) read(e);
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) s[ct][t] = B::mma(k[cb], rows.q[ct][cb], s[ct][t]);
+    for (int e = 0; e < NT * NQB; ++e) {
+      if (e + KEYS_AHEAD - 1 < NT * NQB) read(e + KEYS_AHEAD - 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct][e / NQB] = B::mma(k[e % KEYS_AHEAD], rows.q[ct][e % NQB], s[ct][e / NQB]);
     }
   };
   // A tile's keys are asked for two tiles ahead of its values' product and its values one: while the weights of a tile are worked out from their
@@ -714,20 +722,34 @@ __device__ __forceinline__ void tall_item(Rows<bf16_t, 2>& rows, const Cache<bf1
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = rows.acc[ct][c] * alpha[ct];
     }
+    char* const tile = smem[buffer];
+    if (!whole) {
+      // Values behind the last key become zeros where they lie (every wave does it for itself, all to the same): asked for in the loop below, every
+      // channel tile would wait for its values on its own.
+#pragma unroll 1
+      for (int p = lane; p < 8 * D; p += 64) {
+        float4_t* const at = reinterpret_cast<float4_t*>(tile + TALL_BYTES + (p >> 3) * 128 + 16 * ((p & 7) ^ ((p >> 3) & 7)));
+        float4_t v = *at;
+        B::mask(v, 0, hi - (n0 + 8 * (p & 7)));
+        *at = v;
+      }
+    }
     __builtin_amdgcn_s_setprio(1);
-    const char* const tile = smem[buffer];
+    float4_t v[VALUES_AHEAD][NKB];
+    auto read = [&](int c) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) v[c % VALUES_AHEAD][kb] = *reinterpret_cast<const float4_t*>(tile + (kb ? value_second : value_first) + 2048 * c);
+    };
+#pragma unroll
+    for (int c = 0; c < VALUES_AHEAD - 1; ++c) read(c);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float4_t v[NKB];
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        v[kb] = *reinterpret_cast<const float4_t*>(tile + (kb ? value_second : value_first) + 2048 * c);
-        if (!whole) B::mask(v[kb], 0, hi - (n0 + 32 * kb + 8 * g));
-      }
+      if (c + VALUES_AHEAD - 1 < NC) read(c + VALUES_AHEAD - 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = B::mma(v[kb], pf[ct][kb], rows.acc[ct][c]);
+        for (int ct = 0; ct < CT; ++ct) rows.acc[ct][c] = B::mma(v[c % VALUES_AHEAD][kb], pf[ct][kb], rows.acc[ct][c]);
     }
     __builtin_amdgcn_s_setprio(0);
   };
