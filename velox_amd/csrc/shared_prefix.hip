@@ -25,8 +25,8 @@
 // What bounds them, measured on MI355X (bfloat16, main + joining kernel alone): 48 groups of 5 behind 700 keys (32 heads over 8 of 64 channels, 76 MB) 4.7 + 18.5 +
 // 5.0 us, the stream at 4.1 TB/s in the main one, 2.8 of all three; 8 groups of up to 4 behind 2,048 (28 over 4 of 128, 31 MB) 11.9 + 4.3, four loads that
 // wait for one another and two launches; 64 sequences behind 8,192 (28 over 4, 7.6 GFLOP) 23.4 + 6.5, of which writing and reading the parts' 2 x 24 MB is 8 and
-// half a tile of rows is padding; behind 32,768 (40 over 8, 43 GFLOP) 84.6 to 90 + 8, 0.5 PFLOP/s: exponentials and matrix instructions of two waves a SIMD
-// in turn, at the clock the card holds under them.  4 sequences of 321 keys, taken whole, 8.0 us, in parts it was 7.4 + 3.2 and a launch more.
+// half a tile of rows is padding; behind 32,768 (40 over 8, 43 GFLOP) 80 + 8, 0.54 PFLOP/s: products and weights alone 62, loads alone 46, the
+// sequences' own keys, a third of the bytes, 10.  4 sequences of 321 keys, taken whole, 8.0 us, in parts it was 7.4 + 3.2 and a launch more.
 //
 // Matrix cores: S^T[key, row] = K Q^T and O^T[channel, row] = V^T P^T, both with 16 x 16 results.  For a block of KB contraction
 // indices (32 in bfloat16, 16 in float32) lane (g = lane / 16, i = lane % 16) holds 16 bytes of row or column i, those of place g; a result is rows
