@@ -230,6 +230,16 @@ def test_attention_about_a_waves_lanes(ops, workspace, dtype, groups):
     b.check(b.run(ops, workspace))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("beyond", [0, 1, 7, 8, 9, 33, 63])
+def test_attention_many_rows_of_any_end(ops, workspace, dim, beyond):
+    """Shared keys that end anywhere in a tile; the first sequence has none of its own, and what lies behind its last key is no number."""
+    shared = 4096 + beyond
+    b = Batch(BF16, 8, 2, dim, 16, groups=[(70, shared)], lens=own(70, shared, 0, 40))
+    assert ops._shared_prefix_shape(ops.num_cus, 70, 1, 8, 2, dim, 2, 70, b.longest)[0] == 8
+    b.check(b.run(ops, workspace))
+
+
 def test_attention_without_groups(ops, workspace):
     b = Batch(BF16, 12, 2, 128, 16, groups=[], lens=[100, 1, 333], behind=3)
     b.check(b.run(ops, workspace))
