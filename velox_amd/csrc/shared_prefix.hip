@@ -156,10 +156,18 @@ struct Counts {
   __device__ __forceinline__ int per(const Lengths& l, int steps, int tiles) const {
     return clamped((steps + (tiles + WAVES - 1) / WAVES + l.target - 1) / l.target, 1, MOST_KEYS / 16);  // (nobody has more)
   }
-  // (many rows: `target` workgroups fill the compute units, and the first one more would be a whole round; rounding parts up can bring it about)
-  static constexpr int TRIES = 6;
-  __device__ __forceinline__ bool fills_units(const Lengths& l) const { return l.block_rows > 16 * WAVES; }
-  static __device__ __forceinline__ int raised(int per) { return per + 1 + (per >> 4); }
+  // `target` workgroups are as many as the compute units take in one go, and the first one more takes as long again; rounding parts up can bring it about.
+  // Then somewhat longer parts are tried (of 6 groups of up to 13 behind 10,350 keys, 16 heads over 4, were 72 items for 64 units).
+  // counted(per): the groups' items, or with 0 their blocks
+  template <typename Counted> __device__ __forceinline__ int fitted(const Lengths& l, int per, Counted counted) const {
+    if ((per < 4 && l.block_rows <= 16 * WAVES) || counted(per) <= l.target || counted(0) > l.target) return per;
+    int longer = per;
+    for (int tries = 0; tries < 6; ++tries) {
+      longer += 1 + (longer >> 4);
+      if (counted(longer) <= l.target) return longer;
+    }
+    return per;
+  }
   __device__ __forceinline__ Item of_group(const Lengths& l, int item, int place, int group, int first, int count, int shared, int per) const {
     const int row_blocks = blocks(l, count, shared), part = quotient(place, row_blocks), from = (part * per) << step_shift;
     return Item{group, -1, first, count, place - part * row_blocks, from, min(from + (per << step_shift), shared), item << block_shift};
@@ -199,10 +207,7 @@ __device__ __forceinline__ Item find_item(const Lengths& l, const Counts& counts
 
   const int blocks = counts.blocks(l, end - start, shared), steps = counts.steps(shared), tiles = counts.tiles(own);
   auto sum = [](int v) { return __builtin_amdgcn_readlane(sum_up_to_lane(v), 63); };
-  int per = counts.per(l, sum(blocks * steps), sum(counts.own_blocks * tiles));
-  if (counts.fills_units(l)) {
-    for (int tries = 0; tries < Counts::TRIES && sum(blocks * parts_of(steps, per)) > l.target; ++tries) per = Counts::raised(per);
-  }
+  const int per = counts.fitted(l, counts.per(l, sum(blocks * steps), sum(counts.own_blocks * tiles)), [&](int p) { return sum(p > 0 ? blocks * parts_of(steps, p) : blocks); });
   const int items = blocks * parts_of(steps, per), upto = sum_up_to_lane(items), group_items = __builtin_amdgcn_readlane(upto, 63);
   auto of = [](int v, int at) { return __builtin_amdgcn_readlane(v, at); };
   if (wg < group_items) {
@@ -291,10 +296,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_prefix_plan_kernel(const 
   int tiles = counts.tiles(own);
   for (int b = threads + tid; b < l.num_seqs; b += threads) tiles += counts.tiles(own_of(b, keys_of(b)));
   const Sums work = sums_up_to_thread(blocks * steps, counts.own_blocks * tiles);
-  int per = counts.per(l, work.all_groups, work.all_own);
-  if (counts.fills_units(l)) {
-    for (int tries = 0; tries < Counts::TRIES && sums_up_to_thread(blocks * parts_of(steps, per), 0).all_groups > l.target; ++tries) per = Counts::raised(per);
-  }
+  const int per = counts.fitted(l, counts.per(l, work.all_groups, work.all_own), [&](int p) { return sums_up_to_thread(p > 0 ? blocks * parts_of(steps, p) : blocks, 0).all_groups; });
   const int items = blocks * parts_of(steps, per);
   int group_items = 0, own_items = 0;
   for (int base = 0; base < l.num_seqs; base += threads) {
@@ -775,7 +777,7 @@ template <typename T, int RT> __device__ __forceinline__ void leave_rows(Rows<T,
 }
 
 // Two workgroups to a compute unit where a wave's registers allow it.
-template <typename T, int RT> constexpr int workgroups_per_unit() { return D <= 128 && RT * sizeof(T) * D <= 512 ? 2 : 1; }
+template <typename T, int RT> constexpr int workgroups_per_unit() { return D <= 128 && RT * sizeof(T) * D <= 1024 ? 2 : 1; }
 
 // part_o: [KV head][rows_room][D], part_lse: [KV head][rows_room]; directory: [sequence]
 // RT = TALL: rows in blocks of TALL_ROWS over tiles in LDS.
@@ -802,7 +804,7 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
   float* const o = part_o + (size_t)kvh * l.rows_room * D;
   float* const lse = part_lse + (size_t)kvh * l.rows_room;
   if (item.group >= 0) {
-    if (item.at + R > l.rows_room) return;  // (groups that overlap: no more than there is room for)
+    if (item.at < 0 || item.at + R > l.rows_room) return;  // (groups that overlap: no more than there is room for)
     const int first_row = item.block * R, rows_all = item.count * heads;
     const int* const table = block_tables + (size_t)item.first * table_width;
     auto query_of = [&](int row) -> const T* {
@@ -827,7 +829,7 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
     }
     return;
   }
-  if (item.sequence < 0 || item.at + 16 > l.rows_room) return;
+  if (item.sequence < 0 || item.at < 0 || item.at + 16 > l.rows_room) return;
   Rows<T, 1> rows;
   begin_rows<T, 1>(rows, [&](int r) -> const T* {
     const int row = item.block * 16 + r;

@@ -2335,9 +2335,10 @@ class HipOps:
         Row tiles go by the rows of the largest group: one or two of 16, or eight with tiles of keys in LDS (8).  Measured on MI355X (us, both kernels; 28 heads
         over 4, one group): two / eight with 84 rows behind 8,192 keys 17.2 / 31.5, 224 22.7 / 23.9 and behind 32,768 52 / 49, 336 behind 8,192 33.7 / 28.1, behind 32,768
         102 / 57, 448 behind 1,024 15.6 / 21.0, 4,096 25.2 / 24.8, 32,768 111 / 65; 320 of 64 channels behind 2,048 16.9 / 18.8, 16,384 44.8 / 37.8.  In float32 matrix
-        instructions decide and padded rows cost: one / two row tiles with 48 rows 16.7 / 19.7, 112 37.8 / 40.9, 28 32.3 / 31.2.
-        A workgroup per compute unit but where rows are many or float32 ones are in single tiles, two: one / two with 8 groups of 4 behind 1,024 to 2,048 keys 16.0 / 25.2
-        (more parts to join), 140 rows behind 8,192 19.7 / 22.0; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
+        instructions decide, padded rows cost, and two row tiles pay where a workgroup has many steps; one / two with 48 rows (5 groups behind 1,500) 18.7 / 21.7, 28
+        behind 8,192 20.5 / 25.5, 8 groups of 28 behind 2,048 36.3 / 32.4, 6 of 52 behind 10,350 146 / 120, 70 behind 30,437 73 / 78.
+        A workgroup per compute unit, for many rows two: one / two with 8 groups of 4 behind 1,024 to 2,048 keys 16.0 / 25.2 (more parts to join), 140 rows behind 8,192
+        19.7 / 22.0, in float32 28 behind 8,192 20.5 / 27.7; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
         def refuse():
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences of up to {max_kv_len} keys are more than one call takes")
 
@@ -2350,12 +2351,13 @@ class HipOps:
         row_tiles, per_unit = 1 if rows <= 16 or head_dim > 128 else 2, 1
         if element_size == 2 and head_dim in (64, 128) and rows > 256 and max_kv_len >= 4096:
             row_tiles, per_unit = 8, 2
-        elif element_size == 4 and row_tiles == 2 and -(-rows // 16) % 2 == 1:
-            row_tiles, per_unit = 1, 2
+        elif element_size == 4 and row_tiles == 2:
+            tiles = -(-min(num_groups * rows, num_seqs * group) // 16)  # of all groups
+            row_tiles = 2 if -(-rows // 16) % 2 == 0 and tiles * max_kv_len >= 6 * 64 * (num_cus // num_kv_heads) else 1
         target = max(1, per_unit * num_cus // num_kv_heads)
         block_rows, own_blocks = 16 * row_tiles, num_seqs * (-(-group // 16))
         blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-rows // block_rows))
-        if (own_blocks + blocks) * (max_kv_len // 16 + 2) > 0x7FFFFFFF:  # (tiles of keys are counted in 32 bits)
+        if (own_blocks + num_groups * -(-rows // block_rows)) * (max_kv_len // 16 + 2) > 0x7FFFFFFF:  # (tiles of keys are counted in 32 bits)
             refuse()
         return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
 
