@@ -43,6 +43,8 @@ constexpr int D = VELOX_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head size must be a multiple of 16 between 16 and 256");
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES;
+constexpr int LANE_CHANNELS = D <= 64 ? 1 : D <= 128 ? 2 : 4;                              // of the joining kernel,
+constexpr int JOINED_AT_ONCE = 64 / LANE_CHANNELS < 32 ? 64 / LANE_CHANNELS : 32;          // and parts
 constexpr int MOST_GROUPS = 1024, MOST_KEYS = 1 << 25;  // of a call, of a sequence
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -158,9 +160,14 @@ struct Counts {
   }
   // `target` workgroups are as many as the compute units take in one go, and the first one more takes as long again; rounding parts up can bring it about.
   // Then somewhat longer parts are tried (of 6 groups of up to 13 behind 10,350 keys, 16 heads over 4, were 72 items for 64 units).
-  // counted(per): the groups' items, or with 0 their blocks
-  template <typename Counted> __device__ __forceinline__ int fitted(const Lengths& l, int per, Counted counted) const {
-    if ((per < 4 && l.block_rows <= 16 * WAVES) || counted(per) <= l.target || counted(0) > l.target) return per;
+  static __device__ __forceinline__ bool fills_units(const Lengths& l) { return l.block_rows > 16 * WAVES; }
+  __device__ __forceinline__ int most_parts(const Own& own) const { return tiles(own) + (own.group >= 0 ? steps(own.from) : 0); }
+  // Two steps instead of one make short items twice as long: up to two workgroups a unit then have one each, if that leaves no sequence more parts than the
+  // joining kernel asks for at once (5 groups of up to 8 behind 1,500 float32 keys, 12 heads over 2: 16.7 / 18.2 us; one of 10 behind 2,984 22.0 / 15.2).
+  // counted(per): the groups' items, or with 0 their blocks; most_parts(): a sequence's with a step each
+  template <typename Counted, typename MostParts> __device__ __forceinline__ int fitted(const Lengths& l, int per, Counted counted, MostParts most_parts) const {
+    if (per == 2 && !fills_units(l) && most_parts() <= JOINED_AT_ONCE) return 1;
+    if ((per < 4 && !fills_units(l)) || counted(per) <= l.target || counted(0) > l.target) return per;
     int longer = per;
     for (int tries = 0; tries < 6; ++tries) {
       longer += 1 + (longer >> 4);
@@ -207,7 +214,8 @@ __device__ __forceinline__ Item find_item(const Lengths& l, const Counts& counts
 
   const int blocks = counts.blocks(l, end - start, shared), steps = counts.steps(shared), tiles = counts.tiles(own);
   auto sum = [](int v) { return __builtin_amdgcn_readlane(sum_up_to_lane(v), 63); };
-  const int per = counts.fitted(l, counts.per(l, sum(blocks * steps), sum(counts.own_blocks * tiles)), [&](int p) { return sum(p > 0 ? blocks * parts_of(steps, p) : blocks); });
+  const int per = counts.fitted(l, counts.per(l, sum(blocks * steps), sum(counts.own_blocks * tiles)), [&](int p) { return sum(p > 0 ? blocks * parts_of(steps, p) : blocks); },
+                                [&]() { return __builtin_amdgcn_readlane(most_up_to_lane(counts.most_parts(own)), 63); });
   const int items = blocks * parts_of(steps, per), upto = sum_up_to_lane(items), group_items = __builtin_amdgcn_readlane(upto, 63);
   auto of = [](int v, int at) { return __builtin_amdgcn_readlane(v, at); };
   if (wg < group_items) {
@@ -242,6 +250,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_prefix_plan_kernel(const 
   __shared__ int upto[PLAN_THREADS], from[PLAN_THREADS], to[PLAN_THREADS];
   typedef int two_t __attribute__((ext_vector_type(2)));
   __shared__ two_t wave_sums[2][PLAN_THREADS / 64];
+  __shared__ int most_of[PLAN_THREADS / 64];
   const Counts counts(l, tile_shift, step_shift);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = blockDim.x;  // (as many as there are groups, at least)
   int turn = 0;
@@ -293,10 +302,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_prefix_plan_kernel(const 
     return own_keys(lo, lo >= 0 && b < end[lo] ? shared[lo] : 0, keys);
   };
   Own own = tid < l.num_seqs ? own_of(tid, len0) : Own{-1, 0, 0};
-  int tiles = counts.tiles(own);
-  for (int b = threads + tid; b < l.num_seqs; b += threads) tiles += counts.tiles(own_of(b, keys_of(b)));
+  int tiles = counts.tiles(own), most_parts = counts.most_parts(own);
+  for (int b = threads + tid; b < l.num_seqs; b += threads) {
+    const Own other = own_of(b, keys_of(b));
+    tiles += counts.tiles(other);
+    most_parts = max(most_parts, counts.most_parts(other));
+  }
   const Sums work = sums_up_to_thread(blocks * steps, counts.own_blocks * tiles);
-  const int per = counts.fitted(l, counts.per(l, work.all_groups, work.all_own), [&](int p) { return sums_up_to_thread(p > 0 ? blocks * parts_of(steps, p) : blocks, 0).all_groups; });
+  const int per = counts.fitted(l, counts.per(l, work.all_groups, work.all_own), [&](int p) { return sums_up_to_thread(p > 0 ? blocks * parts_of(steps, p) : blocks, 0).all_groups; },
+                                [&]() {
+                                  const int in_wave = __builtin_amdgcn_readlane(most_up_to_lane(most_parts), 63);
+                                  if (lane == 0) most_of[wave] = in_wave;
+                                  __syncthreads();
+                                  return __builtin_amdgcn_readlane(most_up_to_lane(lane < threads / 64 ? most_of[lane] : 0), 63);
+                                });
   const int items = blocks * parts_of(steps, per);
   int group_items = 0, own_items = 0;
   for (int base = 0; base < l.num_seqs; base += threads) {
@@ -887,15 +906,14 @@ shared_prefix_direct_kernel(const T* __restrict__ qkv, int qkv_stride, const Cac
 }
 
 // A wave per (head, sequence): the parts that hold its row, joined.  Lane p asks for part p's log-sum (the next 64 parts', if there are more, in
-// another round) and every lane for its own channels of up to AHEAD parts, all before it waits for any of them.  A sink adds exp(sink) to the
+// another round) and every lane for its own channels of up to JOINED_AT_ONCE parts, all before it waits for any of them.  A sink adds exp(sink) to the
 // denominator.  (About 4 us for small calls: a launch and three loads in a row; 64 sequences of 28 heads with 27 parts 6.5 us, 24 MB at 3.7 TB/s.)
-constexpr int LANE_CHANNELS = D <= 64 ? 1 : D <= 128 ? 2 : 4, JOIN_HEADS = 4;
+constexpr int JOIN_HEADS = 4;
 template <typename T>
 __global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int nh, int group, int rows_room, const Directory* __restrict__ directory,
                                                                              const float* __restrict__ part_o, const float* __restrict__ part_lse,
                                                                              const float* __restrict__ sinks, T* __restrict__ out) {
   typedef float channels_t __attribute__((ext_vector_type(LANE_CHANNELS)));
-  constexpr int AHEAD = 64 / LANE_CHANNELS < 32 ? 64 / LANE_CHANNELS : 32;
   const int lane = threadIdx.x & 63, head = blockIdx.x * JOIN_HEADS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.y;
   if (head >= nh) return;
   const Directory d = directory[b];
@@ -930,7 +948,7 @@ __global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int
       for (int j = N; j < here; ++j) acc += *reinterpret_cast<const channels_t*>(channels + place_of(p0 + j) * D) * weight_of(j);
     };
     if (here <= 6) join(std::integral_constant<int, 6>{});
-    else join(std::integral_constant<int, AHEAD>{});
+    else join(std::integral_constant<int, JOINED_AT_ONCE>{});
   }
   if (sinks != nullptr && top != -INFINITY) denom += expf(sinks[head] - top);
   if (!live) return;
@@ -949,15 +967,15 @@ extern "C" int velox_shared_prefix_most_row_tiles(int dtype) { return dtype == V
 
 // items: workgroups per KV head, and rows_room: rows per KV head, at least what velox_shared_prefix_room gives.  part_o: float32 [nkv, rows_room, D],
 // part_lse: float32 [nkv, rows_room], directory: eight int32 a sequence.  most_keys: no length counts beyond it.
-// An item has as many steps as the whole over `target`, the last of every row block fewer: at most `target` items and one for every row block, of which
-// the groups have as many as all sequences' rows and one more each fill, or as many each as `largest` sequences do, and the sequences
-// ceil(G / 16) each, a quarter of a workgroup.
+// An item has as many steps as the whole over `target` (or, where that is two, one: twice `target` items then), the last of every row block fewer: at most
+// so many items and one for every row block, of which the groups have as many as all sequences' rows and one more each fill, or as many each
+// as `largest` sequences do, and the sequences ceil(G / 16) each, a quarter of a workgroup.
 extern "C" void velox_shared_prefix_room(int num_seqs, int num_groups, int group, int row_tiles, int target, int largest, long long* items, long long* rows) {
   const long long block_rows = 16LL * row_tiles, own_blocks = (long long)num_seqs * ((group + 15) / 16);
   const long long by_rows = (long long)num_seqs * group / block_rows + num_groups, by_groups = num_groups * (((long long)largest * group + block_rows - 1) / block_rows);
-  const long long blocks = by_rows < by_groups ? by_rows : by_groups;
-  *items = target + blocks + own_blocks / WAVES + 2;
-  *rows = target * (block_rows > 16 * WAVES ? block_rows : 16 * WAVES) + blocks * block_rows + own_blocks * 16 + 16 * WAVES;
+  const long long blocks = by_rows < by_groups ? by_rows : by_groups, most = block_rows > 16 * WAVES ? target : 2LL * target;
+  *items = most + blocks + own_blocks / WAVES + 2;
+  *rows = most * (block_rows > 16 * WAVES ? block_rows : 16 * WAVES) + blocks * block_rows + own_blocks * 16 + 16 * WAVES;
 }
 // What a call brings; the host packs it in this order (one argument costs it less than twenty-eight).
 struct SharedPrefixCall {

@@ -2359,7 +2359,8 @@ class HipOps:
         blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-rows // block_rows))
         if (own_blocks + num_groups * -(-rows // block_rows)) * (max_kv_len // 16 + 2) > 0x7FFFFFFF:  # (tiles of keys are counted in 32 bits)
             refuse()
-        return row_tiles, target, target + blocks + own_blocks // 4 + 2, target * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
+        most = target if row_tiles == 8 else 2 * target
+        return row_tiles, target, most + blocks + own_blocks // 4 + 2, most * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
 
     def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> int:
         """The most float32 elements ``shared_prefix_attention`` asks its workspace for (``shared_prefix_parts``) in any step of at most so many
