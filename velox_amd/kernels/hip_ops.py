@@ -2338,7 +2338,7 @@ class HipOps:
         instructions decide, padded rows cost, and two row tiles pay where a workgroup has many steps; one / two with 48 rows (5 groups behind 1,500) 18.7 / 21.7, 28
         behind 8,192 20.5 / 25.5, 8 groups of 28 behind 2,048 36.3 / 32.4, 6 of 52 behind 10,350 146 / 120, 70 behind 30,437 73 / 78.
         A workgroup per compute unit, for many rows two: one / two with 8 groups of 4 behind 1,024 to 2,048 keys 16.0 / 25.2 (more parts to join), 140 rows behind 8,192
-        19.7 / 22.0, in float32 28 behind 8,192 20.5 / 27.7; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
+        19.7 / 22.0, in float32 28 behind 8,192 20.5 / 27.7, but two where single float32 row tiles have many steps, 2 groups of up to 240 behind 3,200 (40 over 8) 74 / 59; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
         def refuse():
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences of up to {max_kv_len} keys are more than one call takes")
 
@@ -2353,7 +2353,10 @@ class HipOps:
             row_tiles, per_unit = 8, 2
         elif element_size == 4 and row_tiles == 2:
             tiles = -(-min(num_groups * rows, num_seqs * group) // 16)  # of all groups
-            row_tiles = 2 if -(-rows // 16) % 2 == 0 and tiles * max_kv_len >= 6 * 64 * (num_cus // num_kv_heads) else 1
+            if tiles * max_kv_len < 6 * 64 * (num_cus // num_kv_heads):
+                row_tiles = 1
+            elif -(-rows // 16) % 2 == 1:
+                row_tiles, per_unit = 1, 2
         target = max(1, per_unit * num_cus // num_kv_heads)
         block_rows, own_blocks = 16 * row_tiles, num_seqs * (-(-group // 16))
         blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-rows // block_rows))
