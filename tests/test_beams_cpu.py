@@ -121,6 +121,59 @@ def test_attention_items_are_enough(ops, heads, kv_heads, dim):
         assert shared_items * 16 * row_tiles + own_items * 16 <= rows
 
 
+class _Asked(Exception):
+    pass
+
+
+class _Recording:
+    """Says how many elements a call asks for, and ends it."""
+
+    def get(self, name, numel):
+        raise _Asked(numel)
+
+
+def scratch_of_a_call(ops, heads, kv_heads, dim, dtype, num_seqs, num_groups, largest, longest):
+    """Elements that a call of these sizes asks its workspace for."""
+    page = 16
+    call = attention(
+        qkv=torch.empty((num_seqs, heads * dim), dtype=dtype), num_heads=heads, num_kv_heads=kv_heads, head_dim=dim, k_cache=torch.empty((1, kv_heads, page, dim), dtype=dtype),
+        v_cache=torch.empty((1, kv_heads, dim, page), dtype=dtype), block_size=page, block_tables=torch.empty((num_seqs, -(-longest // page)), dtype=torch.int32),
+        kv_lens=torch.empty(num_seqs, dtype=torch.int32), group_starts=torch.empty(num_groups + 1, dtype=torch.int32), shared_lens=torch.empty(num_groups, dtype=torch.int32),
+        largest_group=largest, max_kv_len=longest, workspace=_Recording())
+    try:
+        ops.shared_prefix_attention(**call)
+    except _Asked as asked:
+        return asked.args[0]
+    except AssertionError:
+        return 0  # (the launch was reached: nothing was asked for)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,num_seqs,num_groups,longest", [
+    (12, 2, 128, 81, 1, 32768), (8, 1, 128, 65, 1, 32768), (14, 2, 64, 124, 1, 1000), (12, 2, 128, 210, 1, 1000), (5, 1, 80, 99, 1, 5000),
+])
+def test_attention_scratch_of_large_float32_groups(ops, heads, kv_heads, dim, num_seqs, num_groups, longest):
+    """Single row tiles, two workgroups to a compute unit, items written down ahead."""
+    assert 0 < scratch_of_a_call(ops, heads, kv_heads, dim, torch.float32, num_seqs, num_groups, num_seqs, longest) <= ops.shared_prefix_scratch_elems(heads, kv_heads, dim, num_seqs, num_groups)
+
+
+@pytest.mark.parametrize("num_cus", [256, 64, 304])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(12, 2, 128), (28, 4, 64), (8, 1, 128), (40, 8, 128), (5, 1, 80), (34, 2, 32), (3, 1, 256), (32, 32, 64), (600, 300, 16)])
+def test_attention_scratch_of_any_call_within_limits(ops, heads, kv_heads, dim, num_cus):
+    import random
+
+    rng, ops.num_cus, shared_out = random.Random(heads + num_cus), num_cus, 0
+    for _ in range(60):
+        most_seqs, most_groups = rng.choice([1, 5, 40, 64, 65, 130, 300]), rng.choice([0, 1, 6, 64, 65, 200])
+        most = ops.shared_prefix_scratch_elems(heads, kv_heads, dim, most_seqs, most_groups)
+        for _ in range(4):
+            num_seqs, num_groups = rng.choice([most_seqs, rng.randint(1, most_seqs)]), rng.choice([most_groups, rng.randint(0, most_groups)])
+            asked = scratch_of_a_call(ops, heads, kv_heads, dim, rng.choice([torch.float32, torch.float32, torch.bfloat16]), num_seqs, num_groups,
+                                      rng.choice([num_seqs, rng.randint(1, num_seqs)]), rng.choice([90, 1000, 5000, 32768]))
+            assert asked <= most
+            shared_out += asked > 0
+    assert shared_out > 60
+
+
 @pytest.mark.parametrize("logits,scores,keep,says", [
     (torch.zeros((4, 9), dtype=torch.bfloat16), torch.zeros((2, 2)), 4, "logits"),
     (torch.zeros((4, 9)).double(), torch.zeros((2, 2)), 4, "logits"),

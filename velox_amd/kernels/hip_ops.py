@@ -2357,23 +2357,37 @@ class HipOps:
                 row_tiles = 1
             elif -(-rows // 16) % 2 == 1:
                 row_tiles, per_unit = 1, 2
-        target = max(1, per_unit * num_cus // num_kv_heads)
-        block_rows, own_blocks = 16 * row_tiles, num_seqs * (-(-group // 16))
-        blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-rows // block_rows))
-        if (own_blocks + num_groups * -(-rows // block_rows)) * (max_kv_len // 16 + 2) > 0x7FFFFFFF:  # (tiles of keys are counted in 32 bits)
+        if (num_seqs * (-(-group // 16)) + num_groups * -(-rows // (16 * row_tiles))) * (max_kv_len // 16 + 2) > 0x7FFFFFFF:  # (tiles of keys are counted in 32 bits)
             refuse()
+        target = max(1, per_unit * num_cus // num_kv_heads)
+        return (row_tiles, target) + HipOps._shared_prefix_room(num_seqs, num_groups, group, row_tiles, target, largest_group)
+
+    _SHARED_PREFIX_FORMS = ((1, 1), (1, 2), (2, 1), (8, 2))  # all that ``_shared_prefix_shape`` chooses from: row tiles, workgroups to a compute unit
+
+    @staticmethod
+    def _shared_prefix_room(num_seqs: int, num_groups: int, group: int, row_tiles: int, target: int, largest_group: int) -> Tuple[int, int]:
+        """Workgroups and rows of partial results per KV head at most, as ``velox_shared_prefix_room`` counts them.  (Both grow with the sequences, the groups
+        and the largest group.)"""
+        block_rows, own_blocks = 16 * row_tiles, num_seqs * (-(-group // 16))
+        blocks = min(num_seqs * group // block_rows + num_groups, num_groups * -(-largest_group * group // block_rows))
         most = target if row_tiles == 8 else 2 * target
-        return row_tiles, target, most + blocks + own_blocks // 4 + 2, most * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
+        return most + blocks + own_blocks // 4 + 2, most * max(block_rows, 64) + blocks * block_rows + own_blocks * 16 + 64
+
+    @staticmethod
+    def _shared_prefix_elems(num_seqs: int, num_groups: int, num_kv_heads: int, head_dim: int, items: int, rows: int) -> int:
+        """Float32 elements: partial outputs, their log-sums, where each sequence's rows of them lie, eight numbers, and what each workgroup does, 32 (with up
+        to 64 sequences and groups the workgroups find out for themselves)."""
+        return rows * num_kv_heads * (head_dim + 1) + 8 * num_seqs + (32 * items if num_seqs > 64 or num_groups > 64 else 0)
 
     def shared_prefix_scratch_elems(self, num_heads: int, num_kv_heads: int, head_dim: int, max_num_seqs: int, max_num_groups: int) -> int:
         """The most float32 elements ``shared_prefix_attention`` asks its workspace for (``shared_prefix_parts``) in any step of at most so many
         sequences and groups, whatever the lengths and the element type."""
-        group, rows = num_heads // num_kv_heads, 0
-        for row_tiles in (1, 2, 8):  # (whichever the largest group asks for)
-            blocks, own_blocks = max_num_seqs * group // (16 * row_tiles) + max_num_groups, max_num_seqs * (-(-group // 16))
-            rows = max(rows, max(1, 2 * self.num_cus // num_kv_heads) * max(16 * row_tiles, 64) + blocks * 16 * row_tiles + own_blocks * 16 + 64)
-        items = max(1, 2 * self.num_cus // num_kv_heads) + max_num_seqs * group // 16 + max_num_groups + max_num_seqs * (-(-group // 16)) // 4 + 2
-        return rows * num_kv_heads * (head_dim + 1) + 8 * max_num_seqs + 32 * items
+        most = 0
+        for row_tiles, per_unit in self._SHARED_PREFIX_FORMS:
+            target = max(1, per_unit * self.num_cus // num_kv_heads)
+            items, rows = self._shared_prefix_room(max_num_seqs, max_num_groups, num_heads // num_kv_heads, row_tiles, target, max_num_seqs)
+            most = max(most, self._shared_prefix_elems(max_num_seqs, max_num_groups, num_kv_heads, head_dim, items, rows))
+        return most
 
     def shared_prefix_attention(self, qkv, num_heads, num_kv_heads, head_dim, k_cache, v_cache, block_size, block_tables, kv_lens, group_starts, shared_lens,
                                 largest_group, max_kv_len, scale, workspace, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2434,14 +2448,11 @@ class HipOps:
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences exceed the launch grid")
         directory = parts = planned = sums = 0
         if row_tiles > 0:
-            # partial outputs, their log-sums, where each sequence's rows of them lie, eight numbers, and what each workgroup does, 32 (with up to
-            # 64 sequences and groups the workgroups find out for themselves)
             rows_all = rows * num_kv_heads
-            ahead = num_seqs > 64 or num_groups > 64
-            parts = workspace.get("shared_prefix_parts", rows_all * (head_dim + 1) + 8 * num_seqs + (32 * items if ahead else 0)).data_ptr()
+            parts = workspace.get("shared_prefix_parts", self._shared_prefix_elems(num_seqs, num_groups, num_kv_heads, head_dim, items, rows)).data_ptr()
             sums = parts + 4 * rows_all * head_dim
             directory = sums + 4 * rows_all
-            planned = directory + 32 * num_seqs if ahead else 0
+            planned = directory + 32 * num_seqs if num_seqs > 64 or num_groups > 64 else 0
         call = _SHARED_PREFIX_CALL.pack(
             qkv_at, keys_at, values_at, tables_at, lens_at, starts_at, shared_at, sinks_at, out.data_ptr(), parts, sums, directory, planned,
             rows, items, width, table_width, num_seqs, num_groups, num_heads, num_kv_heads, block_size.bit_length() - 1, pages,
