@@ -649,6 +649,16 @@ def test_reorder_leaves_alone_what_has_no_place(ops):
     check_reorder(ops, [random_rows((9, 50), F32, g)], slots[:0], parents[:0])
 
 
+@pytest.mark.parametrize("width", [64, 7])
+def test_reorder_from_beams_that_take_over_nothing_themselves(ops, width):
+    """A parent may have no parent of its own: its row goes to the others all the same, also where theirs is row 0."""
+    g = torch.Generator().manual_seed(0)
+    slots = torch.tensor([[0, 5, 3, 2], [6, 8, 7, 1]], dtype=torch.int32)
+    for parents in ([[1, -1, 0, 99], [3, 3, -7, -1]], [[2, 2, -1, 2], [1, 4, 1, 1]], [[1, 99, 1, 1], [0, -1, 64, 65]]):
+        check_reorder(ops, [random_rows((9, width), F32, g), random_rows((9, width), BF16, g)], slots, torch.tensor(parents, dtype=torch.int32))
+        check_reorder(ops, [random_rows((9, width), F32, g)], slots.view(2, 2, 2).transpose(0, 1).contiguous(), torch.tensor(parents, dtype=torch.int32).view(2, 4)[:, :2].contiguous())
+
+
 def test_reorder_large_rows(ops):
     """Offsets beyond 32 bits: rows of 96 MiB, seventy of them."""
     rows, width = 70, 24 << 20

@@ -585,7 +585,8 @@ reorder_kernel(const MovedTensors tensors, int count, const int* __restrict__ sl
   }
   const bool there = row >= 0 && row < tensor.rows;
   const uint64_t rows_there = __ballot(there);
-  const bool moves = there && parent >= 0 && parent < beams && (rows_there >> (parent & 63) & 1) != 0 && __shfl(row, parent & 63, VELOX_WAVE) != row;
+  const int source = __shfl(row, parent & 63, VELOX_WAVE);  // (by all lanes: what a lane that stood out had would not be read)
+  const bool moves = there && parent >= 0 && parent < beams && (rows_there >> (parent & 63) & 1) != 0 && source != row;
   uint64_t taken = 0;
   for (uint64_t left = __ballot(moves); left != 0; left &= left - 1) taken |= 1ull << __builtin_amdgcn_readlane(parent, __ffsll((unsigned long long)left) - 1);
   if (taken == 0) return;
