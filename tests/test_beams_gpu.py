@@ -240,6 +240,34 @@ def test_attention_many_rows_of_any_end(ops, workspace, dim, beyond):
     b.check(b.run(ops, workspace))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,groups,own_most", [
+    (16, 4, 64, [(37, 2500)], 150), (16, 4, 128, [(36, 2300), (3, 70), (1, 5)], 700), (8, 8, 32, [(40, 4200), (2, 33)], 60), (32, 8, 96, [(20, 2600)], 90),
+    (12, 2, 128, [(70, 2000)], 120), (12, 2, 128, [(50, 2001), (31, 1000)], 60), (8, 4, 16, [(4, 700), (61, 3100)] + [(2, 90)] * 9, 200), (14, 2, 80, [(13, 4300)] * 6, 40),
+])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_attention_single_float32_row_tiles_of_many_steps(ops, workspace, heads, kv_heads, dim, groups, own_most, sinks):
+    """Two workgroups to a compute unit, with up to 64 sequences and with more; odd and even numbers of row tiles; the same bits every time."""
+    lens = [n for count, shared in groups for n in own(count, shared, 0, own_most)]
+    b = Batch(F32, heads, kv_heads, dim, 16, groups=groups, lens=lens, sinks=sinks, seed=heads)
+    assert ops._shared_prefix_shape(ops.num_cus, len(lens), len(groups), heads, kv_heads, dim, 4, b.largest, b.longest)[:2] == (1, 2 * ops.num_cus // kv_heads)
+    first = b.run(ops, workspace)
+    b.check(first)
+    for _ in range(10):
+        assert torch.equal(first, b.run(ops, workspace))
+
+
+def test_attention_scratch_is_what_it_says_of_many_sequences(ops):
+    """Items written down ahead, in a workspace of the stated size that is fixed."""
+    for heads, kv_heads, dim, groups, own_most in ((12, 2, 128, [(70, 2000)], 120), (8, 4, 16, [(4, 700), (61, 3100)] + [(2, 90)] * 9, 200)):
+        lens = [n for count, shared in groups for n in own(count, shared, 0, own_most)]
+        workspace = Workspace(torch.device("cuda"))
+        workspace.reserve("shared_prefix_parts", ops.shared_prefix_scratch_elems(heads, kv_heads, dim, len(lens), len(groups)))
+        workspace.fix()
+        for dtype in (F32, BF16):
+            b = Batch(dtype, heads, kv_heads, dim, 16, groups=groups, lens=lens)
+            b.check(b.run(ops, workspace))
+
+
 def test_attention_without_groups(ops, workspace):
     b = Batch(BF16, 12, 2, 128, 16, groups=[], lens=[100, 1, 333], behind=3)
     b.check(b.run(ops, workspace))

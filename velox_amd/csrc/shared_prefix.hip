@@ -796,7 +796,7 @@ template <typename T, int RT> __device__ __forceinline__ void leave_rows(Rows<T,
 }
 
 // Two workgroups to a compute unit where a wave's registers allow it.
-template <typename T, int RT> constexpr int workgroups_per_unit() { return D <= 128 && RT * sizeof(T) * D <= 1024 ? 2 : 1; }
+constexpr int workgroups_per_unit() { return D <= 128 ? 2 : 1; }
 
 // part_o: [KV head][rows_room][D], part_lse: [KV head][rows_room]; directory: [sequence]
 // RT = TALL: rows in blocks of TALL_ROWS over tiles in LDS.
@@ -804,7 +804,7 @@ constexpr int TALL = TALL_ROWS / 16;
 template <typename T> constexpr int tile_shift() { return sizeof(T) == 2 ? 5 : 4; }
 template <typename T, int RT> constexpr int step_shift() { return RT == TALL ? 6 : tile_shift<T>() + 2; }
 template <typename T, int RT>
-__global__ void __launch_bounds__(THREADS, (RT == TALL ? 2 : workgroups_per_unit<T, RT>()))
+__global__ void __launch_bounds__(THREADS, (RT == TALL ? 2 : workgroups_per_unit()))
 shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables, int table_width, const Lengths l, float scale,
                      float* __restrict__ part_o, float* __restrict__ part_lse, Directory* __restrict__ directory) {
   constexpr int TILE = Block<T>::KB, R = 16 * RT;
@@ -863,7 +863,7 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
 // join.  What bounds it is latency: a launch (1.6 us), lengths, page ids and keys that wait for one another (0.8 us each), then about 0.7 us for each of a
 // wave's tiles; 4 sequences of 321 keys (12 heads over 2) take 8.0 us.  (With how many keys sharing them out is better: see the host's rule.)
 template <typename T>
-__global__ void __launch_bounds__(THREADS, (workgroups_per_unit<T, 1>()))
+__global__ void __launch_bounds__(THREADS, workgroups_per_unit())
 shared_prefix_direct_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables, int table_width, const Lengths l, float scale,
                             const float* __restrict__ sinks, T* __restrict__ out) {
   constexpr int TILE = Block<T>::KB;
@@ -958,8 +958,9 @@ __global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int
   for (int j = 0; j < LANE_CHANNELS; ++j) dst[j] = from_f32<T>(acc[j]);
 }
 
-// Row tiles a wave can hold: its registers hold the queries, the output and a tile of keys and values.
-template <typename T> constexpr int most_row_tiles() { return D <= 128 ? 2 : 1; }
+// Row tiles a wave can hold: its registers hold the queries, the output and a tile of keys and values.  (In float32 two never pay over more workgroups of one: see the
+// host's rule.)
+template <typename T> constexpr int most_row_tiles() { return sizeof(T) == 2 && D <= 128 ? 2 : 1; }
 
 extern "C" int velox_shared_prefix_head_dim() { return D; }
 extern "C" int velox_shared_prefix_tall(int dtype) { return dtype == VELOX_BF16 && HAS_TALL ? TALL : 0; }

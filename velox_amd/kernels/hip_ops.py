@@ -2334,11 +2334,15 @@ class HipOps:
         12.3 / 10.5, 512 14.0 / 16.5; 240 (960) of 128 27.5 / 25.1, 256 33.6 / 35.4.
         Row tiles go by the rows of the largest group: one or two of 16, or eight with tiles of keys in LDS (8).  Measured on MI355X (us, both kernels; 28 heads
         over 4, one group): two / eight with 84 rows behind 8,192 keys 17.2 / 31.5, 224 22.7 / 23.9 and behind 32,768 52 / 49, 336 behind 8,192 33.7 / 28.1, behind 32,768
-        102 / 57, 448 behind 1,024 15.6 / 21.0, 4,096 25.2 / 24.8, 32,768 111 / 65; 320 of 64 channels behind 2,048 16.9 / 18.8, 16,384 44.8 / 37.8.  In float32 matrix
-        instructions decide, padded rows cost, and two row tiles pay where a workgroup has many steps; one / two with 48 rows (5 groups behind 1,500) 18.7 / 21.7, 28
-        behind 8,192 20.5 / 25.5, 8 groups of 28 behind 2,048 36.3 / 32.4, 6 of 52 behind 10,350 146 / 120, 70 behind 30,437 73 / 78.
+        102 / 57, 448 behind 1,024 15.6 / 21.0, 4,096 25.2 / 24.8, 32,768 111 / 65; 320 of 64 channels behind 2,048 16.9 / 18.8, 16,384 44.8 / 37.8.  Groups of up to 16 rows and
+        heads of more than 128 channels have single ones, and so has float32 (below).
         A workgroup per compute unit, for many rows two: one / two with 8 groups of 4 behind 1,024 to 2,048 keys 16.0 / 25.2 (more parts to join), 140 rows behind 8,192
-        19.7 / 22.0, in float32 28 behind 8,192 20.5 / 27.7, but two where single float32 row tiles have many steps, 2 groups of up to 240 behind 3,200 (40 over 8) 74 / 59; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109."""
+        19.7 / 22.0; of the kernel for many rows 320 behind 32,768 (40 over 8) 161 / 109.
+        In float32 matrix instructions decide: single row tiles, and two workgroups to a unit from six steps (64 keys by 16 rows) a unit on.  Over 244 shapes (heads of 16 to
+        128 channels, groups of 2 to 32 row tiles, 1 to 30 of them, 1,000 to 30,000 keys) the times of single tiles with one workgroup, with two, and of two tiles with one were, relative to
+        the least of the three and on geometric average, 1.03, 1.22 and 1.21 below six steps, 1.09, 1.06 and 1.13 to twelve, 1.08, 1.03 and 1.12 to 24, 1.10, 1.01 and 1.09 beyond (odd and even
+        numbers of tiles alike); one group of 48 rows behind 8,192 (12 over 2, 3.0 steps) 18.6 / 30.1 / 25.5, of 144 behind 30,000 (32 over 8 of 64, 132 steps) 165 / 122 / 154.
+        With groups of up to 16 rows the two are alike (16 groups of 3 behind 3,000, 40 over 8, 97 / 102), and heads of more than 128 channels have registers for one."""
         def refuse():
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences of up to {max_kv_len} keys are more than one call takes")
 
@@ -2348,15 +2352,14 @@ class HipOps:
         if max_kv_len * element_size * max(num_seqs * num_kv_heads * (-(-group // 16)), 2 * num_cus) <= 2048 * num_cus:
             return 0, 1, 0, 0
         rows = largest_group * group
-        row_tiles, per_unit = 1 if rows <= 16 or head_dim > 128 else 2, 1
+        several = rows > 16 and head_dim <= 128
+        row_tiles, per_unit = 2 if several and element_size == 2 else 1, 1
         if element_size == 2 and head_dim in (64, 128) and rows > 256 and max_kv_len >= 4096:
             row_tiles, per_unit = 8, 2
-        elif element_size == 4 and row_tiles == 2:
+        elif element_size == 4 and several:
             tiles = -(-min(num_groups * rows, num_seqs * group) // 16)  # of all groups
-            if tiles * max_kv_len < 6 * 64 * (num_cus // num_kv_heads):
-                row_tiles = 1
-            elif -(-rows // 16) % 2 == 1:
-                row_tiles, per_unit = 1, 2
+            if tiles * max_kv_len >= 6 * 64 * (num_cus // num_kv_heads):
+                per_unit = 2
         if (num_seqs * (-(-group // 16)) + num_groups * -(-rows // (16 * row_tiles))) * (max_kv_len // 16 + 2) > 0x7FFFFFFF:  # (tiles of keys are counted in 32 bits)
             refuse()
         target = max(1, per_unit * num_cus // num_kv_heads)
