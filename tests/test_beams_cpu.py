@@ -1,9 +1,12 @@
 """What the operators for several continuations of one prompt refuse, before anything is launched."""
+import ctypes
 import math
+import random
 
 import pytest
 import torch
 
+from velox_amd.kernels import build
 from velox_amd.kernels.hip_ops import HipOps, KernelError
 
 
@@ -159,8 +162,6 @@ def test_attention_scratch_of_large_float32_groups(ops, heads, kv_heads, dim, nu
 @pytest.mark.parametrize("num_cus", [256, 64, 304])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(12, 2, 128), (28, 4, 64), (8, 1, 128), (40, 8, 128), (5, 1, 80), (34, 2, 32), (3, 1, 256), (32, 32, 64), (600, 300, 16)])
 def test_attention_scratch_of_any_call_within_limits(ops, heads, kv_heads, dim, num_cus):
-    import random
-
     rng, ops.num_cus, shared_out = random.Random(heads + num_cus), num_cus, 0
     for _ in range(60):
         most_seqs, most_groups = rng.choice([1, 5, 40, 64, 65, 130, 300]), rng.choice([0, 1, 6, 64, 65, 200])
@@ -172,6 +173,29 @@ def test_attention_scratch_of_any_call_within_limits(ops, heads, kv_heads, dim, 
             assert asked <= most
             shared_out += asked > 0
     assert shared_out > 60
+
+
+def test_kernels_and_checks_have_the_same_limits(ops):
+    """Also what a call may leave behind, which both sides count."""
+    ops._beams, ops._shared_prefix = None, {}
+    assert ops.beam_library() is not None  # (a library with other limits is refused)
+    lib = ops.shared_prefix_library(64)
+    count, elems = lib.velox_shared_prefix_room, (ctypes.c_longlong * 2)()
+    count.argtypes, count.restype = [ctypes.c_int] * 6 + [ctypes.c_void_p] * 2, None
+    rng = random.Random(3)
+    for _ in range(500):
+        num_seqs, num_groups, group = rng.randint(1, 3000), rng.choice([0, 1, rng.randint(0, 1024)]), rng.choice([1, 2, 7, 16, 17, 64])
+        sizes = num_seqs, num_groups, group, rng.choice([1, 2, 8]), rng.choice([1, 32, 64, 512]), rng.randint(1, num_seqs)
+        count(*sizes, ctypes.addressof(elems), ctypes.addressof(elems) + 8)
+        assert tuple(elems) == ops._shared_prefix_room(*sizes)
+
+
+@pytest.mark.parametrize("changed", ["MAX_BEAMS", "MAX_KEPT", "MAX_BEAM_VOCAB", "MAX_MOVED", "MAX_MOVED_TENSORS", "MAX_PREFIX_GROUPS", "MAX_PREFIX_KEYS"])
+def test_a_library_of_other_limits_is_refused(ops, changed):
+    ops._beams, ops._shared_prefix = None, {}
+    setattr(ops, changed, getattr(ops, changed) + 1)
+    with pytest.raises(KernelError, match="other limits"):
+        ops.shared_prefix_library(64) if "PREFIX" in changed else ops.beam_library()
 
 
 @pytest.mark.parametrize("logits,scores,keep,says", [

@@ -963,8 +963,12 @@ __global__ void __launch_bounds__(64 * JOIN_HEADS) shared_prefix_join_kernel(int
 template <typename T> constexpr int most_row_tiles() { return sizeof(T) == 2 && D <= 128 ? 2 : 1; }
 
 extern "C" int velox_shared_prefix_head_dim() { return D; }
-extern "C" int velox_shared_prefix_tall(int dtype) { return dtype == VELOX_BF16 && HAS_TALL ? TALL : 0; }
-extern "C" int velox_shared_prefix_most_row_tiles(int dtype) { return dtype == VELOX_BF16 ? most_row_tiles<bf16_t>() : most_row_tiles<float>(); }
+extern "C" int velox_shared_prefix_most_groups() { return MOST_GROUPS; }
+extern "C" int velox_shared_prefix_most_keys() { return MOST_KEYS; }
+static bool has_row_tiles(int row_tiles, int dtype) {  // 0: all keys in one workgroup
+  if (row_tiles < 0 || (row_tiles & (row_tiles - 1)) != 0) return false;
+  return row_tiles <= (dtype == VELOX_BF16 ? most_row_tiles<bf16_t>() : most_row_tiles<float>()) || (row_tiles == TALL && dtype == VELOX_BF16 && HAS_TALL);
+}
 
 // items: workgroups per KV head, and rows_room: rows per KV head, at least what velox_shared_prefix_room gives.  part_o: float32 [nkv, rows_room, D],
 // part_lse: float32 [nkv, rows_room], directory: eight int32 a sequence.  most_keys: no length counts beyond it.
@@ -1029,8 +1033,7 @@ extern "C" int velox_shared_prefix_attention(const SharedPrefixCall* call, hipSt
   if (c.num_seqs <= 0) return 0;
   if (c.nkv < 1 || c.nh < 1 || c.nh % c.nkv != 0 || c.page_shift < 3 || c.page_shift > 16 || c.pages < 1 || c.most_keys < 0 || c.most_keys > MOST_KEYS || c.most_keys > (long long)c.table_width << c.page_shift ||
       c.num_groups < 0 || c.num_groups > MOST_GROUPS || c.target < 1 || c.largest < 1 || c.largest > c.num_seqs || c.num_seqs > 65535 || c.items > 65535 || c.rows_room > 0x7fffffffLL) return -1;
-  if (c.row_tiles < 0 || (c.row_tiles & (c.row_tiles - 1)) != 0 ||
-      (c.row_tiles > velox_shared_prefix_most_row_tiles(c.dtype) && c.row_tiles != velox_shared_prefix_tall(c.dtype))) return -1;
+  if (!has_row_tiles(c.row_tiles, c.dtype)) return -1;
   const int group = c.nh / c.nkv;
   if (c.row_tiles > 0) {
     long long least_items, least_rows;

@@ -284,11 +284,12 @@ class HipOps:
         if lib is None:
             lib = ctypes.CDLL(build.ensure_shared_prefix(head_dim))
             lib.velox_shared_prefix_attention.argtypes = [ctypes.c_char_p, _P]
-            lib.velox_shared_prefix_most_row_tiles.argtypes = [_I]
-            for fn in (lib.velox_shared_prefix_attention, lib.velox_shared_prefix_most_row_tiles, lib.velox_shared_prefix_head_dim):
+            for fn in (lib.velox_shared_prefix_attention, lib.velox_shared_prefix_head_dim, lib.velox_shared_prefix_most_groups, lib.velox_shared_prefix_most_keys):
                 fn.restype = _I
             if lib.velox_shared_prefix_head_dim() != head_dim:
                 raise KernelError(f"shared-prefix library for head_dim={head_dim} reports {lib.velox_shared_prefix_head_dim()}")
+            if (lib.velox_shared_prefix_most_groups(), lib.velox_shared_prefix_most_keys()) != (self.MAX_PREFIX_GROUPS, self.MAX_PREFIX_KEYS):
+                raise KernelError("the kernels of shared_prefix_attention have other limits than its checks")
             self._shared_prefix[head_dim] = lib
         return lib
 
@@ -300,8 +301,11 @@ class HipOps:
             lib.velox_beam_scratch_bytes.restype = ctypes.c_longlong
             lib.velox_beam_select.argtypes = [_P, _P, _I, _I, _I, _I, _I, _P, ctypes.c_longlong, _P, _P]
             lib.velox_reorder_states.argtypes = [_P, _I, _P, _P, _I, _I, _I, _P]
-            for fn in (lib.velox_beam_select, lib.velox_reorder_states):
+            limits = (lib.velox_beam_most_beams, lib.velox_beam_most_kept, lib.velox_beam_most_vocab, lib.velox_reorder_most_beams, lib.velox_reorder_most_tensors)
+            for fn in (lib.velox_beam_select, lib.velox_reorder_states) + limits:
                 fn.restype = _I
+            if tuple(fn() for fn in limits) != (self.MAX_BEAMS, self.MAX_KEPT, self.MAX_BEAM_VOCAB, self.MAX_MOVED, self.MAX_MOVED_TENSORS):
+                raise KernelError("the kernels of beam_select and reorder_states have other limits than their checks")
             self._beams = lib
         return self._beams
 
@@ -2319,7 +2323,7 @@ class HipOps:
     # -- several continuations of one prompt ------------------------------------------------------
     MAX_PREFIX_GROUPS, MAX_PREFIX_KEYS = 1024, 1 << 25  # of one call of ``shared_prefix_attention``, of a sequence in it
     MAX_BEAMS, MAX_KEPT, MAX_BEAM_VOCAB = 256, 64, 1 << 24  # of ``beam_select``
-    MAX_MOVED = 64  # beams of a request that ``reorder_states`` moves
+    MAX_MOVED, MAX_MOVED_TENSORS = 64, 32  # beams of a request that ``reorder_states`` moves, tensors of one of its launches
 
     @staticmethod
     @functools.lru_cache(maxsize=4096)
@@ -2536,9 +2540,9 @@ class HipOps:
             return
         launch = self.beam_library().velox_reorder_states
         at = 0
-        while at < len(described):  # up to 32 tensors and 65,535 runs of rows a launch
+        while at < len(described):  # up to so many tensors and 65,535 runs of rows a launch
             end, runs = at, 0
-            while end < len(described) and end - at < 32 and runs + described[end][1] <= 65535:
+            while end < len(described) and end - at < self.MAX_MOVED_TENSORS and runs + described[end][1] <= 65535:
                 runs += described[end][1]
                 end += 1
             numbers = array.array("q", [n for d in described[at:end] for n in d])
