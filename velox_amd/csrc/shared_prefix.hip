@@ -115,7 +115,11 @@ struct Lengths {
 struct Own { int group, from, to; };  // a sequence's own keys [from, to); group: whose shared keys it has, or -1
 
 __device__ __forceinline__ int clamped(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
-// a / b rounded down, 0 <= a < 2^23 <= 2^31 / b: by the reciprocal, which is off by one at most
+// a / b rounded down, 0 <= a < 2^23, 1 <= b < 2^23, a / b < 2^22: by the reciprocal.  a and b are exact in 32 bits, the reciprocal is off by 2^-23 of it at most and the
+// product by 2^-24 of it, the estimate so by less than 0.75, after rounding down by one at most; q b lies within b of a.
+// Divided are a sequence's steps or tiles of keys and what an item has of them, together, by the latter (2^21 of either at most, an item's half more where parts
+// are fitted to the units), and an item's place among those of its group or sequence, which a launch's 65,535 workgroups of four waves hold.
+static_assert(MOST_KEYS / 16 * 5 / 2 < 1 << 23 && MOST_KEYS / 16 < 1 << 22 && WAVES * 65535 < 1 << 22, "numbers that the quotient takes");
 __device__ __forceinline__ int quotient(int a, int b) {
   int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
   const int rest = a - q * b;
