@@ -13,11 +13,12 @@
 // exception; a list that is full is cut to its best `keep`.  The waves read what bounds the others have published and wait for one
 // another behind the first round alone.
 //
-// What bounds it, measured on MI355X: 512 rows of 152,064 tokens (64 requests of 8 beams, 311 MB) 83 us and 7 for joining, 3.7 TB/s.  The same from the
-// second-level cache alone takes 72 us, without the exponentials 34; from memory without them 60: vector instructions, 28 a logit, of which the exponential in 64
+// What bounds it, measured on MI355X: 512 rows of 152,064 tokens (64 requests of 8 beams, 311 MB) take 85 to 88 us a call, 3.6 TB/s; traced, where kernels are slower, 95 us
+// (median of 30 calls, the least 88) and 7.6 for joining.  Variants of it were timed untraced, this kernel 83 us then: the same from the
+// second-level cache alone 72 us, without the exponentials 34; from memory without them 60: vector instructions, 28 a logit, of which the exponential in 64
 // bits is 16, and a stream that reaches 5.4 TB/s overlap by half.  (In 32 bits it would be 63 us, and the sums 1e-7 off where 6e-11 settles the order of near
-// ones.)  64 rows of 152,064 21 + 6 us, 168 of 32,003 17 + 11, 4 of 151,936 8 + 6: of these, launches, the first round, in which much joins the
-// lists, and the lists' joining are most.
+// ones.)  Medians of traced calls, both kernels: 64 rows of 152,064 22.6 + 6.2 us, 168 of 32,003 18.8 + 11.4, 4 of 151,936 8.2 + 7.0: of these, launches, the first round, in
+// which much joins the lists, and the lists' joining are most.
 //
 // reorder_states: row slots[b, j, p] of every tensor becomes what row slots[b, parents[b, j], p] was.  A thread owns a column of the rows of one
 // request: it has read all that move before it writes any, and nobody else reads or writes that column, so the rows change places

@@ -8,7 +8,8 @@
 //
 // for any split point P: each part gives its own o and log-sum l, and o = sum_i exp(l_i) o_i / sum_i exp(l_i).  The first part's keys
 // are the same for the group's sequences, so n_g G rows of queries stand against one stream of keys and values, which is read
-// once; the second part is each sequence's own, G rows against its keys.
+// once for every block of 16 (float32, and heads of more than 128 channels), 32 or 128 of them; the second part is each sequence's own, G rows
+// against its keys.
 //
 // Four kernels; which ones a call takes goes by its sizes (the host's rules):
 //
@@ -22,11 +23,12 @@
 // this one's have been multiplied, its values as soon as this one's have, two workgroups to a compute unit.  With many rows the products
 // count, and the waves share tiles in LDS instead (tall_item).
 //
-// What bounds them, measured on MI355X (bfloat16, main + joining kernel alone): 48 groups of 5 behind 700 keys (32 heads over 8 of 64 channels, 76 MB) 4.7 + 18.5 +
-// 5.0 us, the stream at 4.1 TB/s in the main one, 2.8 of all three; 8 groups of up to 4 behind 2,048 (28 over 4 of 128, 31 MB) 11.9 + 4.3, four loads that
-// wait for one another and two launches; 64 sequences behind 8,192 (28 over 4, 7.6 GFLOP) 23.4 + 6.5, of which writing and reading the parts' 2 x 24 MB is 8 and
-// half a tile of rows is padding; behind 32,768 (40 over 8, 43 GFLOP) 80 + 8, 0.54 PFLOP/s: products and weights alone 62, loads alone 46, the
-// sequences' own keys, a third of the bytes, 10.  4 sequences of 321 keys, taken whole, 8.0 us, in parts it was 7.4 + 3.2 and a launch more.
+// What bounds them, measured on MI355X (bfloat16; medians of 30 traced calls, kernel by kernel: an untraced call takes up to a tenth less than their sum): 48 groups of 5
+// behind 700 keys (32 heads over 8 of 64 channels, 76 MB) 5.2 + 18.8 + 4.9 us, the stream at 4.0 TB/s in the main one, 2.6 of all three; 8 groups of up to 4 behind 2,048 (28
+// over 4 of 128, 31 MB) 12.0 + 4.3, four loads that wait for one another and two launches; 64 sequences behind 8,192 (28 over 4, 7.6 GFLOP) 24.6 + 6.5, of which writing and
+// reading the parts' 2 x 24 MB is 8 and half a tile of rows is padding; behind 32,768 (40 over 8, 43 GFLOP) 86.6 + 8.3 (81 a call untraced, 0.53 PFLOP/s): products and weights
+// alone 62, loads alone 46, the sequences' own keys, a third of the bytes, 10, of untraced copies.  4 sequences of 321 keys, taken whole, 8.3 us, in parts it was 7.4 + 3.2 and
+// a launch more.
 //
 // Matrix cores: S^T[key, row] = K Q^T and O^T[channel, row] = V^T P^T, both with 16 x 16 results.  For a block of KB contraction
 // indices (32 in bfloat16, 16 in float32) lane (g = lane / 16, i = lane % 16) holds 16 bytes of row or column i, those of place g; a result is rows
@@ -865,7 +867,7 @@ shared_prefix_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> c
 
 // Few keys: a workgroup per (KV head, sequence, 16 of its rows) takes all of them, the shared ones too, and leaves the result itself: no plan, no parts, nothing to
 // join.  What bounds it is latency: a launch (1.6 us), lengths, page ids and keys that wait for one another (0.8 us each), then about 0.7 us for each of a
-// wave's tiles; 4 sequences of 321 keys (12 heads over 2) take 8.0 us.  (With how many keys sharing them out is better: see the host's rule.)
+// wave's tiles; 4 sequences of 321 keys (12 heads over 2) take 8.3 us (traced).  (With how many keys sharing them out is better: see the host's rule.)
 template <typename T>
 __global__ void __launch_bounds__(THREADS, workgroups_per_unit())
 shared_prefix_direct_kernel(const T* __restrict__ qkv, int qkv_stride, const Cache<T> cache, const int* __restrict__ block_tables, int table_width, const Lengths l, float scale,

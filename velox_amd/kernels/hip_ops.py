@@ -2398,17 +2398,22 @@ class HipOps:
 
     def shared_prefix_attention(self, qkv, num_heads, num_kv_heads, head_dim, k_cache, v_cache, block_size, block_tables, kv_lens, group_starts, shared_lens,
                                 largest_group, max_kv_len, scale, workspace, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Attention of a decode step whose sequences share their first keys in groups: the shared keys are read once per group, and not once per
-        sequence as by ``paged_attention``, whose arguments these are otherwise.  One token per sequence (row ``b`` of ``qkv``).
+        """Attention of a decode step whose sequences share their first keys in groups: the shared keys are read for many of a group's sequences at a time,
+        and not for each of them as by ``paged_attention``.  One token per sequence (row ``b`` of ``qkv``).  ``qkv`` to ``block_tables``, ``scale`` and
+        ``sinks`` are as there; its windows, biases by distance, kept tokens, capped scores and gates are not taken, nor is latent attention.
 
-        Group ``g`` is sequences ``group_starts[g] .. group_starts[g + 1] - 1`` (int32 ``[groups + 1]``, rising); the first ``shared_lens[g]``
-        keys (int32 ``[groups]``; any number, pages need not be full) of each of them are the same ones, and are read through
+        Group ``g`` is sequences ``group_starts[g] .. group_starts[g + 1] - 1`` (int32 ``[groups + 1]``, rising; in any other order the outputs are unspecified); the
+        first ``shared_lens[g]`` keys (int32 ``[groups]``; any number, pages need not be full) of each of them are the same ones, and are read through
         the block table of the group's FIRST sequence.  What a sequence has behind them is read through its own table, whose entries for
         pages that hold shared keys only are not looked at.  Sequences outside every group, alone in one, or with fewer keys than their group
         shares share nothing; a group shares no more keys than its first sequence has.  A sequence without keys gets zeros.
         ``largest_group``: at least the sequences of the largest group (what a group has beyond shares nothing either), ``max_kv_len``: the most keys
         of any sequence (a greater length counts as that many).  Lengths and groups are read on the device only: a captured call replays with other ones, as long as the number of
-        sequences and groups stays.  ``sinks``: as for ``paged_attention``.  Pages hold 8 to 65,536 tokens."""
+        sequences and groups stays.  Pages hold 8 to 65,536 tokens.
+
+        How often the shared keys are read: once for every 32 rows (a row: one sequence's query head, those of a KV head counted) of a group in bfloat16, 16
+        in float32 and for heads of more than 128 channels, 128 in bfloat16 for heads of 64 and 128 channels where the largest group has more than 256 rows and ``max_kv_len``
+        is 4,096 or more (one choice for all groups of a call).  In short steps (``_shared_prefix_shape``) every sequence reads them for itself."""
         num_seqs, num_groups = kv_lens.numel(), shared_lens.numel()
         dtype = qkv.dtype
         element_size = 2 if dtype == torch.bfloat16 else 4
@@ -2476,10 +2481,11 @@ class HipOps:
 
     def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, keep: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """The ``keep`` best continuations of every request over its beams and the vocabulary.  ``logits`` float32 ``[requests * beams, vocab]``,
-        ``scores`` float32 ``[requests, beams]``, the beams' sums of log-probabilities (-inf: a beam that is not there).  A continuation of beam ``w``
+        ``scores`` float32 ``[requests, beams]``, the beams' sums of log-probabilities.  A continuation of beam ``w``
         by token ``v`` is worth ``scores[w] + log_softmax(logits[w])[v]``, in 64 bits.  Returns, best first, their values (float32), their beams
         and their tokens (int32), each ``[requests, keep]``.  Equal ones come by the lowest beam, then by the greater logit, then by the lowest token;
-        a logit that is -inf or no number makes a value of -inf, and those come last."""
+        a logit that is -inf or no number makes a value of -inf, and those come last.  A beam whose score is -inf or no number is not there: its
+        logits are not looked at, all its values are -inf, and its continuations come by the lowest token."""
         if logits.dim() != 2 or scores.dim() != 2 or scores.numel() != logits.shape[0]:
             raise KernelError(f"beam_select: {tuple(scores.shape)} scores do not go with logits of shape {tuple(logits.shape)}")
         (requests, beams), (rows, vocab), keep = scores.shape, logits.shape, int(keep)
