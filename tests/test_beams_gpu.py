@@ -435,6 +435,40 @@ def test_attention_captured_of_many_sequences(ops):
             b.check(eager)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("count,shared,own_most", [(3, 100, 30), (4, 900, 200), (70, 4100, 40)])
+def test_attention_pages_beyond_32_bits(ops, workspace, dtype, count, shared, own_most):
+    """The same bits from pages whose offsets in bytes and in elements pass 32 bits."""
+    b = Batch(dtype, 8, 2, 128, 16, groups=[(count, shared)], lens=own(count, shared, 1, own_most))
+    longest = b.most_keys if shared < 200 else b.longest  # (few keys are taken whole)
+    want = b.run(ops, workspace, longest=longest)
+    b.check(want)
+    pages = b.k.shape[0]
+    many = 2 ** 32 // (2 * 16 * 128) + pages + 1  # (2^32 elements and more)
+    k, v = torch.empty((many,) + b.k.shape[1:], dtype=dtype, device="cuda"), torch.empty((many,) + b.v.shape[1:], dtype=dtype, device="cuda")
+    k[many - pages:], v[many - pages:] = b.k, b.v
+    b.k, b.v, b.tables = k, v, b.tables + (many - pages)
+    assert torch.equal(b.run(ops, workspace, longest=longest), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("count,shared,own_most", [(3, 100, 30), (4, 900, 200), (40, 3000, 60), (70, 4100, 40)])
+def test_attention_infinite_values(ops, workspace, dtype, count, shared, own_most):
+    """An infinite value makes its channel infinite for those who see it, not a number that is none, and nothing else."""
+    b = Batch(dtype, 8, 2, 64, 16, groups=[(count, shared)], lens=own(count, shared, 2, own_most), spread=0.2)
+    b.longest = max(b.most_keys, 1050) if shared > 200 else b.most_keys
+    want = b.run(ops, workspace).view(count, 2, 4, 64)
+    for key in (0, shared - 1):
+        b.v[b.tables[0, key // 16].long(), 1, 7, key % 16] = math.inf  # (a shared key of the second KV head)
+    last = b.lens[2].item() - 1
+    b.v[b.tables[2, last // 16].long(), 0, 5, last % 16] = -math.inf  # (one of the third sequence's own, of the first)
+    got = b.run(ops, workspace).view(count, 2, 4, 64)
+    assert (got[:, 1, :, 7] == math.inf).all() and (got[2, 0, :, 5] == -math.inf).all()
+    rest = torch.ones_like(got, dtype=torch.bool)
+    rest[:, 1, :, 7] = rest[2, 0, :, 5] = False
+    assert torch.equal(got[rest], want[rest])
+
+
 def test_attention_on_another_stream(ops, workspace):
     b = Batch(BF16, 12, 2, 128, 16, groups=[(6, 700)], lens=own(6, 700, 1, 200))
     want = b.run(ops, workspace)
