@@ -2345,7 +2345,7 @@ class HipOps:
         In float32 matrix instructions decide: single row tiles, and two workgroups to a unit from six steps (64 keys by 16 rows) a unit on.  Over 244 shapes (heads of 16 to
         128 channels, groups of 2 to 32 row tiles, 1 to 30 of them, 1,000 to 30,000 keys) the times of single tiles with one workgroup, with two, and of two tiles with one were, relative to
         the least of the three and on geometric average, 1.03, 1.22 and 1.21 below six steps, 1.09, 1.06 and 1.13 to twelve, 1.08, 1.03 and 1.12 to 24, 1.10, 1.01 and 1.09 beyond (odd and even
-        numbers of tiles alike); one group of 48 rows behind 8,192 (12 over 2, 3.0 steps) 18.6 / 30.1 / 25.5, of 144 behind 30,000 (32 over 8 of 64, 132 steps) 165 / 122 / 154.
+        numbers of tiles alike; a shape by itself is up to 19% faster or 27% slower than with two tiles, with no size that tells which: how evenly items come out decides); one group of 48 rows behind 8,192 (12 over 2, 3.0 steps) 18.6 / 30.1 / 25.5, of 144 behind 30,000 (32 over 8 of 64, 132 steps) 165 / 122 / 154.
         With groups of up to 16 rows the two are alike (16 groups of 3 behind 3,000, 40 over 8, 97 / 102), and heads of more than 128 channels have registers for one."""
         def refuse():
             raise KernelError(f"shared_prefix_attention: {num_seqs} sequences of up to {max_kv_len} keys are more than one call takes")
